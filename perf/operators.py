@@ -1,0 +1,369 @@
+"""Cases of the key/value cache operators: appending tokens to a paged 8-bit cache, and attention that reads it.
+
+The cache of one attention layer: pages of `page` tokens, every (page, head) block of K and of V held as e4m3 codes
+beside one power-of-two scale 2^e (e8m0), value = code * 2^e.  A batch is packed row-wise: rows
+[row_start[b], row_start[b + 1]) belong to sequence b, whose cache holds kv_len[b] tokens with those rows as the last
+ones, in the pages that row b of page_table lists.
+
+  append: k -> RMSNorm (per head, optional) -> rotation by the position's (cos, sin) row (optional) -> block scale and
+          codes; v -> block scale and codes; q (optional) -> RMSNorm -> rotation -> bf16.  e is the smallest integer
+          with absmax <= 448 * 2^e in [-60, 60]; a block that keeps earlier tokens never lowers its e, and when e
+          grows the kept codes are rounded to it.
+  attend: softmax(q k^T / sqrt(128)) v over the tokens a row sees: the first hi = kv_len - rows + i + 1 of them for
+          row i of a causal call and all kv_len otherwise, of those the last `window` when there is one; a row that
+          sees nothing gives zeros.  Query head h reads cache head h / (heads / kv_heads).
+
+Codes come back in their own 8-bit type with the scales beside them: together they are the values that the cache
+stands for, and that pair is what a program holds.
+"""
+import math
+
+import torch
+
+own = False
+
+D = 128
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+EMIN, EMAX = -60, 60
+
+
+# ------------------------------------------------------------------------------------------------ cases
+
+def _attend(name, seqs, rows, kv, heads, kv_heads, page, causal=True, window=0):
+    return dict(name=name, op="attend", seqs=seqs, rows=rows, kv=kv, heads=heads, kv_heads=kv_heads, page=page,
+                causal=causal, window=window)
+
+
+def _append(name, seqs, rows, kv, heads, kv_heads, page, norm=True, rope=True, with_q=True):
+    return dict(name=name, op="append", seqs=seqs, rows=rows, kv=kv, heads=heads, kv_heads=kv_heads, page=page,
+                norm=norm, rope=rope, with_q=with_q)
+
+
+def listed():
+    return [
+        # one new token against one latent frame of a 12-head video model: nothing but latency
+        _attend("attend 1x1 kv1561 h12", 1, 1, 1561, 12, 12, 64),
+        # an ordinary serving step: a ragged batch, four query heads to a cache head
+        _attend("attend 32x1 kv4097 h32/8", 32, 1, 4097, 32, 8, 64),
+        # the same far into long contexts: the cache is what is read
+        _attend("attend 64x1 kv16384 h32/8", 64, 1, 16384, 32, 8, 64),
+        # one very long sequence with as many cache heads as query heads: few rows, one long axis
+        _attend("attend 1x1 kv131071 h40", 1, 1, 131071, 40, 40, 64),
+        # a few draft tokens at a time behind a sliding window, small pages, an odd head ratio
+        _attend("attend 8x5 kv20000 w4096 h28/4", 8, 5, 20000, 28, 4, 16, window=4096),
+        # a frame of 480 x 832 video (1560 tokens) over the seven frames so far: no mask, compute-bound
+        _attend("attend 1x1560 kv10920 h40", 1, 1560, 10920, 40, 40, 64, causal=False),
+        # prompts of different lengths, causal, grouped heads
+        _attend("attend 3x4096 kv5001 h32/8", 3, 4096, 5001, 32, 8, 128),
+        # three frames at once over twenty-one: the largest
+        _attend("attend 1x4680 kv32760 h40", 1, 4680, 32760, 40, 40, 64, causal=False),
+        # one token of one sequence: nothing but latency
+        _append("append 1x1 kv1561 h12", 1, 1, 1561, 12, 12, 64),
+        # a serving step
+        _append("append 32x1 kv4097 h32/8", 32, 1, 4097, 32, 8, 64),
+        # prompts of different lengths; pages end inside them
+        _append("append 8x2001 kv3001 h32/8", 8, 2001, 3001, 32, 8, 128),
+        # three frames of a 40-head video model, keys normalised and rotated over all heads beforehand
+        _append("append 1x4680 kv32760 h40", 1, 4680, 32760, 40, 40, 64, norm=False, rope=False, with_q=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kv_heads = rng.choice((1, 2, 4, 5, 8, 12, 24, 40))
+    group = rng.choice((1, 1, 2, 4, 5, 7, 8)) if kv_heads <= 8 else 1
+    page = rng.choice((16, 32, 64, 128))
+    kind = rng.choice(("token", "token", "draft", "chunk", "append", "append"))
+    if kind == "append":
+        seqs = _log(rng, 1, 64)
+        rows = _log(rng, 1, max(1, min(4680, 20000 // seqs)))
+        kv = rows + rng.randrange(0, 5000)
+        return dict(op="append", seqs=seqs, rows=rows, kv=kv, heads=kv_heads * group, kv_heads=kv_heads, page=page,
+                    norm=rng.random() < 0.6, rope=rng.random() < 0.7, with_q=rng.random() < 0.6)
+    if kind == "token" or kind == "draft":
+        seqs = _log(rng, 1, 64)
+        most = 16384 * 64 * 8 // (seqs * kv_heads)
+        kv = _log(rng, 1, max(2, min(131071, most)))
+        rows = 1 if kind == "token" else rng.randrange(2, 17)
+    else:
+        seqs = rng.randrange(1, 5)
+        rows = _log(rng, 17, 4680 * 40 // (seqs * max(40, kv_heads * group)))
+        kv = min(32760, rows + _log(rng, 1, 28000 // seqs))
+    causal = kind != "chunk" or rng.random() < 0.5
+    window = _log(rng, 1, kv) if rng.random() < 0.25 else 0
+    return dict(op="attend", seqs=seqs, rows=rows, kv=kv, heads=kv_heads * group, kv_heads=kv_heads, page=page,
+                causal=causal, window=window)
+
+
+def _lengths(case):
+    """(rows, tokens after the rows) of every sequence: the first has the case's own, the others spread below them."""
+    rows, kv = [], []
+    for b in range(case["seqs"]):
+        r = case["rows"] - (b * 7919) % (case["rows"] // 2 + 1)
+        t = case["kv"] - (b * 104729) % (case["kv"] // 2 + 1)
+        rows.append(r)
+        kv.append(max(t, r) if case["op"] == "append" else max(t, 1))
+    return rows, kv
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+
+def _block_exponent(amax):
+    """Smallest integer e in [EMIN, EMAX] with amax <= 448 * 2^e (448 = 0.875 * 2^9)."""
+    m, x = torch.frexp(amax)
+    e = torch.where(m <= 0.875, x - 9, x - 8)
+    return torch.where(amax > 0, e, EMIN).clamp(EMIN, EMAX)
+
+
+def _codes(pages, heads, page, spread, g):
+    """A pool of pages as a running program leaves it: normal values, a magnitude per (page, head)."""
+    codes = torch.empty((pages, heads, page, D), dtype=E4M3, device="cuda")
+    exps = torch.empty((pages, heads), dtype=torch.int32, device="cuda")
+    step = max(1, (1 << 27) // (heads * page * D))
+    for p in range(0, pages, step):
+        n = min(step, pages - p)
+        x = torch.randn((n, heads, page, D), generator=g, device="cuda")
+        if spread:
+            x *= torch.exp(spread * torch.randn((n, heads, 1, 1), generator=g, device="cuda"))
+        e = _block_exponent(x.abs().amax((2, 3)))
+        codes[p:p + n] = torch.ldexp(x, -e[:, :, None, None]).to(E4M3)
+        exps[p:p + n] = e
+    return codes, (exps + 127).to(torch.uint8).view(E8M0)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows, kv = _lengths(case)
+    hq, hkv, page = case["heads"], case["kv_heads"], case["page"]
+    held = [-(-n // page) for n in kv]
+    pool = sum(held) + 3
+    where = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(kv), max(held)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(held):
+        table[b, :n] = where[at:at + n]
+        at += n
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    s = dict(case=case, table=table, row_start=torch.tensor(starts, dtype=torch.int32, device="cuda"),
+             kv_len=torch.tensor(kv, dtype=torch.int32, device="cuda"))
+    s["k_cache"], s["k_scale"] = _codes(pool, hkv, page, 0.0, g)
+    s["v_cache"], s["v_scale"] = _codes(pool, hkv, page, 0.5, g)
+    total = starts[-1]
+    if case["op"] == "attend":
+        s["q"] = (2.0 * torch.randn((total, hq, D), generator=g, device="cuda")).bfloat16()
+    else:
+        # q, k and v heads side by side, as one projection of the rows leaves them
+        packed = torch.randn((total, hq + 2 * hkv, D), generator=g, device="cuda").bfloat16()
+        s["q"] = packed[:, :hq] if case["with_q"] else None
+        s["k"], s["v"] = packed[:, hq:hq + hkv], packed[:, hq + hkv:]
+        weight = lambda: (1 + 0.1 * torch.randn(D, generator=g, device="cuda")).bfloat16()  # noqa: E731
+        s["k_norm_w"] = weight() if case["norm"] else None
+        s["q_norm_w"] = weight() if case["norm"] and case["with_q"] else None
+        s["rope"] = None
+        if case["rope"]:
+            freq = 10000.0 ** (-torch.arange(0, D, 2, device="cuda", dtype=torch.float64) / D)
+            angle = torch.arange(max(kv), device="cuda", dtype=torch.float64)[:, None] * freq
+            s["rope"] = torch.stack((angle.cos(), angle.sin()), -1).float()[None]
+    if own:
+        from diffsynth_engine_amd import kv_cache
+
+        s["cache"] = kv_cache.KVCache(s["k_cache"], s["v_cache"], s["k_scale"], s["v_scale"])
+        s["plan"] = kv_cache.KVPlan(table, s["row_start"], s["kv_len"], max_rows=max(rows), max_kv_len=max(kv))
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+
+def _exponents(scale):
+    return scale.view(torch.uint8).to(torch.int32) - 127
+
+
+def _placed(s, total):
+    """For every packed row its sequence and its position in it."""
+    row = torch.arange(total, device="cuda")
+    seq = torch.searchsorted(s["row_start"][1:].long(), row, right=True)
+    count = s["row_start"].diff()
+    return seq, row - s["row_start"][seq], (s["kv_len"] - count)[seq] + row - s["row_start"][seq]
+
+
+def _norm_rope(x, weight, rope, pos):
+    x = x.float()
+    if weight is not None:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * weight.float()
+    if rope is not None:
+        c, t = rope[0, pos, :, 0][:, None], rope[0, pos, :, 1][:, None]
+        a, b = x[..., 0::2], x[..., 1::2]
+        x = torch.stack((a * c - b * t, a * t + b * c), -1).flatten(-2)
+    return x
+
+
+def _store(s, x, codes, scale, seq, pos):
+    page = s["case"]["page"]
+    pool, heads = scale.shape
+    start = s["kv_len"] - s["row_start"].diff()
+    first = s["table"].gather(1, (start // page).clamp(max=s["table"].shape[1] - 1)[:, None].long())[:, 0].long()
+    kept = torch.where(s["row_start"].diff() > 0, start % page, 0)  # tokens that stay in a sequence's first block
+    block, off = s["table"][seq, pos // page].long(), pos % page
+    amax = torch.zeros((pool, heads), device="cuda")
+    amax.index_reduce_(0, block, x.abs().amax(-1), "amax")
+    old = _exponents(scale)
+    new = _block_exponent(amax)
+    new[first] = torch.where(kept[:, None] > 0, torch.maximum(new[first], old[first]), new[first])
+    held = codes.view(torch.uint8)[first].view(E4M3).float()
+    moved = torch.ldexp(held, (old - new)[first][:, :, None, None]).to(E4M3).float()
+    stays = torch.arange(page, device="cuda") < kept[:, None]
+    codes.view(torch.uint8)[first] = torch.where(stays[:, None, :, None], moved, held).to(E4M3).view(torch.uint8)
+    q = torch.ldexp(x, -new[block][..., None]).clamp(-448, 448).to(E4M3)
+    codes.view(torch.uint8)[block, :, off] = q.view(torch.uint8)
+    scale.view(torch.uint8)[block] = (new[block] + 127).to(torch.uint8)
+
+
+def _plain_append(s):
+    seq, _, pos = _placed(s, s["k"].shape[0])
+    _store(s, _norm_rope(s["k"], s["k_norm_w"], s["rope"], pos), s["k_cache"], s["k_scale"], seq, pos)
+    _store(s, s["v"].float(), s["v_cache"], s["v_scale"], seq, pos)
+    return None if s["q"] is None else _norm_rope(s["q"], s["q_norm_w"], s["rope"], pos).bfloat16()
+
+
+def _gathered(s, codes, scale):
+    at = s["table"].clamp(min=0).long()
+    x = codes.view(torch.uint8)[at].view(E4M3).float()  # (sequences, pages, heads, page, D)
+    x = torch.ldexp(x, _exponents(scale)[at][..., None, None])
+    return x.transpose(1, 2).flatten(2, 3)
+
+
+def _plain_attend(s):
+    case = s["case"]
+    q, hkv = s["q"], case["kv_heads"]
+    total, hq, _ = q.shape
+    g = hq // hkv
+    count = s["row_start"].diff()
+    seq, i, _ = _placed(s, total)
+    most = case["rows"]
+    at = (s["row_start"][:-1, None] + torch.arange(most, device="cuda")).clamp(max=total - 1)
+    qs = q[at].float().unflatten(2, (hkv, g)).permute(0, 2, 1, 3, 4).flatten(2, 3)  # (sequences, hkv, most * g, D)
+    k, v = _gathered(s, s["k_cache"], s["k_scale"]), _gathered(s, s["v_cache"], s["v_scale"])
+    key = torch.arange(k.shape[2], device="cuda")
+    end = s["kv_len"][:, None].expand(-1, most)
+    if case["causal"]:
+        end = (s["kv_len"] - count)[:, None] + torch.arange(most, device="cuda") + 1
+    begin = end - case["window"] if case["window"] else torch.zeros_like(end)
+    seen = (key < end[..., None]) & (key >= begin[..., None])
+    seen = seen.repeat_interleave(g, 1)[:, None]
+    x = torch.matmul(qs, k.transpose(2, 3))
+    x.mul_(1 / math.sqrt(D)).masked_fill_(~seen, -math.inf)
+    top = x.amax(-1, keepdim=True)
+    x.sub_(top.masked_fill(top == -math.inf, 0.0)).exp_()
+    o = torch.matmul(x, v) / x.sum(-1, keepdim=True).clamp(min=1e-30)
+    o = o.unflatten(2, (most, g)).permute(0, 2, 1, 3, 4).flatten(2, 3)
+    return o[seq, i].bfloat16()
+
+
+def run(s):
+    if s["case"]["op"] == "append":
+        if own:
+            from diffsynth_engine_amd import ops
+
+            q = ops.kv_append(s["k"], s["v"], s["cache"], s["plan"], k_norm_w=s["k_norm_w"], rope=s["rope"], q=s["q"],
+                              q_norm_w=s["q_norm_w"])
+        else:
+            q = _plain_append(s)
+        return dict(q=q, k=s["k_cache"], v=s["v_cache"], k_scale=s["k_scale"], v_scale=s["v_scale"])
+    if own:
+        from diffsynth_engine_amd import ops
+
+        return ops.kv_attention(s["q"], s["cache"], s["plan"], causal=s["case"]["causal"], window=s["case"]["window"])
+    return _plain_attend(s)
+
+
+# ------------------------------------------------------------------------------------------------ work, exact values
+
+def work(case):
+    rows, kv = _lengths(case)
+    hq, hkv, page = case["heads"], case["kv_heads"], case["page"]
+    total = sum(rows)
+    meta = 4 * (2 * len(rows) + 1 + sum(-(-n // page) for n in kv))
+    if case["op"] == "append":
+        heads = 2 * hkv + (2 * hq if case["with_q"] else 0)  # what is read; q goes out as wide as it came
+        size = 2 * total * D * heads + 2 * total * D * hkv + 2 * sum(-(-r // page) for r in rows) * hkv + meta
+        size += 8 * (D // 2) * min(max(kv), total) if case["rope"] else 0
+        each = (4 if case["norm"] else 0) + (3 if case["rope"] else 0)
+        return dict(bytes=size, flops=total * D * (hkv * (each + 4) + (hq * each if case["with_q"] else 0)))
+    pairs = keys = 0
+    for r, n in zip(rows, kv):
+        ends = [n - r + i + 1 for i in range(r)] if case["causal"] else [n] * r
+        spans = [(max(0, e - case["window"]) if case["window"] else 0, e) for e in ends if e > 0]
+        pairs += sum(e - b for b, e in spans)
+        keys += max(e for _, e in spans) - min(b for b, _ in spans) if spans else 0
+    return dict(bytes=4 * total * hq * D + 2 * keys * hkv * D + 2 * -(-keys // page) * hkv + meta,
+                flops=4 * pairs * hq * D)
+
+
+def _exact_side(s, b, x, codes, exps, first, n):
+    """The blocks of sequence b that its rows x (rows, heads, D) reach, tokens [first, n) of it."""
+    page = s["case"]["page"]
+    for p in range(first // page, -(-n // page)):
+        lo, hi = max(first, p * page), min(n, (p + 1) * page)
+        at, kept = int(s["table"][b, p]), lo - p * page
+        part = x[lo - first:hi - first]
+        top = part.abs().amax((0, 2))
+        e = torch.ceil(torch.log2(top / 448)).clamp(EMIN, EMAX)
+        if kept:
+            e = torch.maximum(e, exps[at])
+            codes[at, :, :kept] *= 2.0 ** (exps[at] - e)[:, None, None]
+        codes[at, :, kept:kept + hi - lo] = (part / 2.0 ** e[None, :, None]).transpose(0, 1)
+        exps[at] = e
+
+
+def _turned(x, weight, rope, first):
+    x = x.double()
+    if weight is not None:
+        x = x / torch.sqrt((x * x).sum(-1, keepdim=True) / D + 1e-6) * weight.double()
+    if rope is None:
+        return x
+    z = torch.view_as_complex(x.unflatten(-1, (D // 2, 2)).contiguous())
+    turn = torch.view_as_complex(rope[0, first:first + x.shape[0]].double().contiguous())
+    return torch.view_as_real(z * turn[:, None]).flatten(-2)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    rows, kv = _lengths(case)
+    hkv = case["kv_heads"]
+    starts = s["row_start"].tolist()
+    if case["op"] == "append":
+        out = {n: s[n + "_cache"].double() for n in "kv"}
+        exps = {n: _exponents(s[n + "_scale"]).double() for n in "kv"}
+        q = None if s["q"] is None else torch.empty(s["q"].shape, dtype=torch.float64, device="cuda")
+        for b, (r, n) in enumerate(zip(rows, kv)):
+            part = slice(starts[b], starts[b + 1])
+            _exact_side(s, b, _turned(s["k"][part], s["k_norm_w"], s["rope"], n - r), out["k"], exps["k"], n - r, n)
+            _exact_side(s, b, s["v"][part].double(), out["v"], exps["v"], n - r, n)
+            if q is not None:
+                q[part] = _turned(s["q"][part], s["q_norm_w"], s["rope"], n - r)
+        return dict(q=q, k=out["k"], v=out["v"], k_scale=2.0 ** exps["k"], v_scale=2.0 ** exps["v"])
+    o = torch.empty(s["q"].shape, dtype=torch.float64, device="cuda")
+    g = case["heads"] // hkv
+    for b, (r, n) in enumerate(zip(rows, kv)):
+        pages = s["table"][b, :-(-n // case["page"])].long()
+        end = torch.full((r,), n, device="cuda")
+        if case["causal"]:
+            end = n - r + 1 + torch.arange(r, device="cuda")
+        key = torch.arange(n, device="cuda")
+        hidden = key[None] >= end[:, None]
+        if case["window"]:
+            hidden |= key[None] < (end - case["window"])[:, None]
+        for h in range(hkv):
+            kh, vh = (torch.mul(s[c + "_cache"].view(torch.uint8)[pages, h].view(E4M3).double(),
+                                2.0 ** _exponents(s[c + "_scale"])[pages, h].double()[:, None, None]).reshape(-1, D)[:n]
+                      for c in "kv")
+            for j in range(h * g, (h + 1) * g):
+                x = (s["q"][starts[b]:starts[b + 1], j].double() @ kh.T / D ** 0.5).masked_fill(hidden, -math.inf)
+                p = torch.softmax(x, -1).masked_fill(hidden, 0.0)
+                o[starts[b]:starts[b + 1], j] = p @ vh
+    return o
