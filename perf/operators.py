@@ -7,7 +7,7 @@ ones, in the pages that row b of page_table lists.
 
   append: k -> RMSNorm (per head, optional) -> rotation by the position's (cos, sin) row (optional) -> block scale and
           codes; v -> block scale and codes; q (optional) -> RMSNorm -> rotation -> bf16.  e is the smallest integer
-          with absmax <= 448 * 2^e in [-60, 60]; a block that keeps earlier tokens never lowers its e, and when e
+          with absmax <= 448 * 2^e in [-48, 48]; a block that keeps earlier tokens never lowers its e, and when e
           grows the kept codes are rounded to it.
   attend: softmax(q k^T / sqrt(128)) v over the tokens a row sees: the first hi = kv_len - rows + i + 1 of them for
           row i of a causal call and all kv_len otherwise, of those the last `window` when there is one; a row that
@@ -24,7 +24,7 @@ own = False
 
 D = 128
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
-EMIN, EMAX = -60, 60
+EMIN, EMAX = -48, 48
 
 
 # ------------------------------------------------------------------------------------------------ cases
