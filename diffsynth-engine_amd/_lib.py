@@ -77,6 +77,56 @@ class GemmProblem(ctypes.Structure):
     ]
 
 
+class KVCacheParams(ctypes.Structure):
+    """Mirror of ``dsx_kv_cache``."""
+
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("k_sp", c_int64), ("k_sh", c_int64), ("v_sp", c_int64), ("v_sh", c_int64),
+        ("ks_sp", c_int64), ("vs_sp", c_int64),
+        ("pages", ctypes.c_int32), ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class KVBatchParams(ctypes.Structure):
+    """Mirror of ``dsx_kv_batch``."""
+
+    _fields_ = [
+        ("page_table", c_void_p), ("table_sb", c_int64),
+        ("row_start", c_void_p), ("kv_len", c_void_p),
+        ("batch", ctypes.c_int32), ("table_pages", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32), ("max_kv_len", ctypes.c_int32),
+    ]
+
+
+class KVAppendParams(ctypes.Structure):
+    """Mirror of ``dsx_kv_append_params``."""
+
+    _fields_ = [
+        ("k", c_void_p), ("k_sr", c_int64), ("k_sh", c_int64),
+        ("v", c_void_p), ("v_sr", c_int64), ("v_sh", c_int64),
+        ("q", c_void_p), ("q_sr", c_int64), ("q_sh", c_int64),
+        ("q_out", c_void_p), ("qo_sr", c_int64), ("qo_sh", c_int64),
+        ("k_norm_w", c_void_p), ("q_norm_w", c_void_p),
+        ("rope", c_void_p), ("rope_sb", c_int64), ("rope_rows", c_int64),
+        ("total_rows", c_int64),
+        ("norm_eps", c_float), ("heads_q", ctypes.c_int32),
+    ]
+
+
+class KVAttnParams(ctypes.Structure):
+    """Mirror of ``dsx_kv_attn_params``."""
+
+    _fields_ = [
+        ("q", c_void_p), ("q_sr", c_int64), ("q_sh", c_int64),
+        ("out", c_void_p), ("o_sr", c_int64), ("o_sh", c_int64),
+        ("total_rows", c_int64),
+        ("softmax_scale", c_float), ("heads_q", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 GEMM_GROUP_MAX = 4
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares
@@ -120,6 +170,10 @@ SIGNATURES = {
     "dsx_gelu_erf": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                              c_void_p]),
     "dsx_flow_match_euler_step": (c_int, [c_void_p, c_void_p, c_float, c_void_p, c_int64, c_int, c_void_p]),
+    "dsx_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dsx_kv_attn": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dsx_kv_attn_workspace_bytes": (c_int64, [c_void_p, c_void_p, c_void_p]),
+    "dsx_kv_plan_check": (c_int, [c_void_p, ctypes.c_int32, ctypes.c_int32, c_int64, c_int, c_void_p]),
     "dsx_mfma_ceiling_probe": (c_int, [c_int, c_void_p, c_int64, ctypes.c_int32, c_void_p, ctypes.POINTER(c_int64),
                                        c_void_p]),
 }

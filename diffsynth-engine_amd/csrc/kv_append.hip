@@ -1,0 +1,305 @@
+// Appending a batch's keys and values to the paged 8-bit cache, and its queries' normalisation and rotation.
+//
+// One workgroup = one (page, head) block of K or of V, or 64 (row, head) pairs of q.  A block's tokens are held in
+// registers between the two passes over them (largest magnitude, then codes), so each element is read once and written
+// once: 16 lanes per token, 8 elements per lane, page/16 tokens per lane.
+#include <stdlib.h>
+
+#include "kv_internal.h"
+
+namespace dsx {
+namespace {
+
+struct AppendArgs {
+  dsx_kv_cache c;
+  dsx_kv_batch n;
+  dsx_kv_append_params p;
+  int page_shift;
+  int blocks_per_seq;  // pages that max_rows rows can reach
+  int64_t q_begin;     // first workgroup of the q part
+  int q_per_seq;
+};
+
+__device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a token
+  v += dpp_f32<kDppRowRor8>(v);
+  v += dpp_f32<kDppRowRor4>(v);
+  v += dpp_f32<kDppQuadXor2>(v);
+  v += dpp_f32<kDppQuadXor1>(v);
+  return v;
+}
+
+__device__ __forceinline__ void load8(const uint16_t* src, float (&x)[8]) {
+  const u32x4 w = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = bf16_lo(w[j]);
+    x[2 * j + 1] = bf16_hi(w[j]);
+  }
+}
+
+// RMSNorm over the head, then the rotation of pairs (2i, 2i + 1): lane `ln` of the token's 16 holds elements 8 ln ..
+__device__ __forceinline__ void norm_rope(float (&x)[8], const uint16_t* w, float eps, const float* rope_row, int ln) {
+  if (w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+    const float r = 1.0f / sqrtf(row16_sum(ss) * (1.0f / kKvDim) + eps);
+    float g[8];
+    load8(w + 8 * ln, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= r * g[j];
+  }
+  if (rope_row) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln);
+    const f32x4 b = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln + 4);
+    const float cs[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x0 = x[2 * j], x1 = x[2 * j + 1], c = cs[2 * j], s = cs[2 * j + 1];
+      x[2 * j] = x0 * c - x1 * s;
+      x[2 * j + 1] = x0 * s + x1 * c;
+    }
+  }
+}
+
+// value * 2^-e as the clamp's operand: saturates at +-448 (infinities too), NaN stays NaN
+__device__ __forceinline__ float clamp448(float v) {
+  const float y = fminf(fmaxf(v, -448.f), 448.f);
+  return v == v ? y : v;
+}
+
+template <int TOK>  // tokens per 16-lane group = page / 16
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
+  const dsx_kv_cache& c = a.c;
+  const dsx_kv_batch& n = a.n;
+  const dsx_kv_append_params& p = a.p;
+  const int tid = threadIdx.x, ln = tid & 15, grp = tid >> 4;
+  __shared__ uint32_t smax[4];
+
+  if ((int64_t)blockIdx.x >= a.q_begin) {
+    const int64_t u = (int64_t)blockIdx.x - a.q_begin;
+    const int b = (int)(u / a.q_per_seq), chunk = (int)(u % a.q_per_seq);
+    const KvSeq s = kv_seq(n, b, p.total_rows);
+    if (!s.ok || s.kv < s.rows) return;
+    const int64_t pairs = (int64_t)s.rows * p.heads_q;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int64_t pr = (int64_t)chunk * 64 + it * 16 + grp;
+      if (pr >= pairs) return;
+      const int row = (int)(pr / p.heads_q), h = (int)(pr % p.heads_q);
+      float x[8];
+      load8((const uint16_t*)p.q + (int64_t)(s.row0 + row) * p.q_sr + h * p.q_sh + 8 * ln, x);
+      const float* rr = p.rope ? p.rope + b * p.rope_sb + (int64_t)(s.kv - s.rows + row) * kKvDim : nullptr;
+      norm_rope(x, (const uint16_t*)p.q_norm_w, p.norm_eps, rr, ln);
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+      *reinterpret_cast<u32x4*>((uint16_t*)p.q_out + (int64_t)(s.row0 + row) * p.qo_sr + h * p.qo_sh + 8 * ln) = w;
+    }
+    return;
+  }
+
+  // ---- one (page, head) block of K or V
+  unsigned u = blockIdx.x;
+  const int h = (int)(u % c.heads);
+  u /= c.heads;
+  const bool is_v = u & 1;
+  u >>= 1;
+  const int j = (int)(u % a.blocks_per_seq), b = (int)(u / a.blocks_per_seq);
+  const KvSeq s = kv_seq(n, b, p.total_rows);
+  if (!s.ok || s.kv < s.rows) return;
+  const int first = s.kv - s.rows;  // the first appended token
+  const int page = c.page_size;
+  const int pi = (first >> a.page_shift) + j;
+  const int base = pi << a.page_shift;  // the block's first token
+  if (base >= s.kv || s.rows == 0) return;
+  const int id = n.page_table[b * n.table_sb + pi];
+  if (id < 0 || id >= c.pages) return;
+  const int lo = first > base ? first - base : 0;  // tokens [lo, hi) of the block are new, [0, lo) stay
+  const int hi = s.kv - base < page ? s.kv - base : page;
+
+  const uint16_t* src = is_v ? (const uint16_t*)p.v + h * p.v_sh : (const uint16_t*)p.k + h * p.k_sh;
+  const int64_t sr = is_v ? p.v_sr : p.k_sr;
+  uint8_t* codes = is_v ? (uint8_t*)c.v + id * c.v_sp + h * c.v_sh : (uint8_t*)c.k + id * c.k_sp + h * c.k_sh;
+  uint8_t* scale = is_v ? (uint8_t*)c.v_scale + id * c.vs_sp + h : (uint8_t*)c.k_scale + id * c.ks_sp + h;
+
+  float x[TOK][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < TOK; ++i) {
+    const int t = grp + 16 * i;
+    if (t >= lo && t < hi) {
+      load8(src + (int64_t)(s.row0 + base + t - first) * sr + 8 * ln, x[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+    }
+  }
+  if (!is_v && (p.k_norm_w || p.rope)) {
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const int t = grp + 16 * i;
+      const float* rr = p.rope && t >= lo && t < hi ? p.rope + b * p.rope_sb + (int64_t)(base + t) * kKvDim : nullptr;
+      norm_rope(x[i], (const uint16_t*)p.k_norm_w, p.norm_eps, rr, ln);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TOK; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = fabsf(x[i][e]);
+      amax = fmaxf(amax, v < INFINITY ? v : 0.f);
+    }
+  amax = wave_max(amax);
+  if ((tid & 63) == 0) smax[tid >> 6] = __float_as_uint(amax);  // (non-negative floats order as their bits)
+  __syncthreads();
+  const uint32_t top = max(max(smax[0], smax[1]), max(smax[2], smax[3]));
+  int e = kv_block_exponent(top);
+  if (lo > 0) {
+    const int old = (int)*scale - 127;
+    if (old > e) {
+      e = old;
+    } else if (old < e) {  // the kept codes move to the larger scale: exact but for what becomes subnormal
+#pragma unroll
+      for (int i = 0; i < TOK; ++i) {
+        const int t = grp + 16 * i;
+        if (t < lo) {
+          u32x2* at = reinterpret_cast<u32x2*>(codes + t * kKvDim + 8 * ln);
+          u32x2 w = *at;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            float f[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f[q] = ldexpf(e4m3_bits_to_f32((w[d] >> (8 * q)) & 0xffu), old - e);
+            w[d] = pack_e4m3x4_inrange(f[0], f[1], f[2], f[3]);
+          }
+          *at = w;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TOK; ++i) {
+    const int t = grp + 16 * i;
+    if (t >= lo && t < hi) {
+      u32x2 w;
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        float f[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f[q] = clamp448(ldexpf(x[i][4 * d + q], -e));
+        w[d] = pack_e4m3x4_inrange(f[0], f[1], f[2], f[3]);
+      }
+      *reinterpret_cast<u32x2*>(codes + t * kKvDim + 8 * ln) = w;
+    }
+  }
+  __syncthreads();  // every lane has read the old exponent
+  if (tid == 0) *scale = (uint8_t)(e + 127);
+}
+
+bool rows_ok(const void* p, int64_t sr, int64_t sh) { return ((uintptr_t)p & 15) == 0 && sr % 8 == 0 && sh % 8 == 0; }
+
+}  // namespace
+
+int kv_check_cache(const dsx_kv_cache* c, const dsx_kv_batch* n, int64_t total_rows) {
+  if (!c || !n) return DSX_ENULL;
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale || !n->page_table || !n->row_start || !n->kv_len) return DSX_ENULL;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return DSX_EBADSHAPE;
+  if (c->pages < 1 || c->heads < 1 || n->batch < 1 || n->table_pages < 1 || n->table_sb < n->table_pages ||
+      n->max_rows < 0 || n->max_rows > (1 << 30) || n->max_kv_len < 0 || n->max_kv_len > (1 << 30) || total_rows < 0 ||
+      total_rows > 0x7fffffff || n->max_kv_len > (int64_t)n->table_pages * c->page_size)
+    return DSX_EBADSHAPE;
+  if (c->k_sp % 16 || c->k_sh % 16 || c->v_sp % 16 || c->v_sh % 16) return DSX_EALIGN;
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return DSX_EALIGN;
+  if (((uintptr_t)n->page_table | (uintptr_t)n->row_start | (uintptr_t)n->kv_len) & 3) return DSX_EALIGN;
+  return DSX_OK;
+}
+
+}  // namespace dsx
+
+extern "C" int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const dsx_kv_append_params* p,
+                             void* stream) {
+  using namespace dsx;
+  if (!p) return DSX_ENULL;
+  const int rc = kv_check_cache(cache, batch, p->total_rows);
+  if (rc != DSX_OK) return rc;
+  const dsx_kv_cache& c = *cache;
+  const dsx_kv_batch& n = *batch;
+  if (!p->k || !p->v || (p->q && !p->q_out)) return DSX_ENULL;
+  if (p->q && p->heads_q < 1) return DSX_EBADSHAPE;
+  if (!(p->norm_eps >= 0.f)) return DSX_EBADSHAPE;
+  if (!rows_ok(p->k, p->k_sr, p->k_sh) || !rows_ok(p->v, p->v_sr, p->v_sh)) return DSX_EALIGN;
+  if (p->q && (!rows_ok(p->q, p->q_sr, p->q_sh) || !rows_ok(p->q_out, p->qo_sr, p->qo_sh))) return DSX_EALIGN;
+  if (((uintptr_t)p->k_norm_w | (uintptr_t)p->q_norm_w | (uintptr_t)p->rope) & 15) return DSX_EALIGN;
+  if (p->rope && (p->rope_rows < n.max_kv_len || p->rope_sb % 4 ||
+                  (p->rope_sb != 0 && p->rope_sb < p->rope_rows * kKvDim)))
+    return DSX_EBADSHAPE;
+  if (n.max_rows == 0 || p->total_rows == 0) return DSX_OK;
+  AppendArgs a{};
+  a.c = c;
+  a.n = n;
+  a.p = *p;
+  a.page_shift = __builtin_ctz((unsigned)c.page_size);
+  const int64_t rows = n.max_rows < n.max_kv_len ? n.max_rows : n.max_kv_len;
+  if (rows == 0) return DSX_OK;
+  a.blocks_per_seq = (int)((rows + c.page_size - 2) / c.page_size + 1);
+  const int64_t kv_wgs = (int64_t)n.batch * a.blocks_per_seq * c.heads * 2;
+  a.q_begin = kv_wgs;
+  const int64_t q_per_seq = p->q ? (rows * p->heads_q + 63) / 64 : 0;
+  const int64_t total = kv_wgs + (int64_t)n.batch * q_per_seq;
+  if (total >= (1ll << 31) || q_per_seq >= (1ll << 31)) return DSX_EBADSHAPE;
+  a.q_per_seq = (int)q_per_seq;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)total), block(256);
+  switch (c.page_size) {
+    case 16: kv_append_kernel<1><<<grid, block, 0, st>>>(a); break;
+    case 32: kv_append_kernel<2><<<grid, block, 0, st>>>(a); break;
+    case 64: kv_append_kernel<4><<<grid, block, 0, st>>>(a); break;
+    default: kv_append_kernel<8><<<grid, block, 0, st>>>(a); break;
+  }
+  return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;
+}
+
+extern "C" int dsx_kv_plan_check(const dsx_kv_batch* n, int32_t pages, int32_t page_size, int64_t total_rows,
+                                 int for_append, int32_t* bad_sequence) {
+  using namespace dsx;
+  if (!n || !n->page_table || !n->row_start || !n->kv_len) return DSX_ENULL;
+  if (page_size < 1 || pages < 1 || n->batch < 1 || n->table_pages < 1 || n->table_sb < n->table_pages)
+    return DSX_EBADSHAPE;
+  int32_t none;
+  int32_t& bad = bad_sequence ? *bad_sequence : none;
+  for (int b = 0; b < n->batch; ++b) {
+    bad = b;
+    const KvSeq s = kv_seq(*n, b, total_rows);
+    if (!s.ok || s.kv > (int64_t)n->table_pages * page_size) return DSX_EBADSHAPE;
+    if (for_append && s.kv < s.rows) return DSX_EBADSHAPE;
+    const int32_t* row = n->page_table + b * n->table_sb;
+    for (int t = 0; t < ((int64_t)s.kv + page_size - 1) / page_size; ++t)
+      if (row[t] < 0 || row[t] >= pages) return DSX_EBADSHAPE;
+  }
+  if (for_append) {  // a page that is written belongs to one place of one sequence
+    uint8_t* listed = (uint8_t*)calloc((size_t)pages, 1);
+    if (!listed) return DSX_EWORKSPACE;
+    int rc = DSX_OK;
+    for (int pass = 0; pass < 2 && rc == DSX_OK; ++pass)
+      for (int b = 0; b < n->batch && rc == DSX_OK; ++b) {
+        const KvSeq s = kv_seq(*n, b, total_rows);
+        const int32_t* row = n->page_table + b * n->table_sb;
+        const int end = (int)(((int64_t)s.kv + page_size - 1) / page_size);
+        const int begin = pass == 0 ? 0 : s.rows == 0 ? end : (s.kv - s.rows) / page_size;
+        for (int t = begin; t < end; ++t) {
+          uint8_t& times = listed[row[t]];
+          if (pass == 0) {
+            times = times < 2 ? times + 1 : 2;
+          } else if (times > 1) {
+            bad = b;
+            rc = DSX_EBADSHAPE;
+          }
+        }
+      }
+    free(listed);
+    if (rc != DSX_OK) return rc;
+  }
+  bad = -1;
+  return DSX_OK;
+}

@@ -1,0 +1,546 @@
+// Attention over the paged 8-bit key/value cache.
+//
+// Work: a unit is (sequence, cache head, block of query rows), where the query rows of a cache head are its
+// heads_q / heads query heads times the sequence's rows, packed as row * group + head.  A workgroup walks a piece of the
+// unit's key range in tiles of 32 keys, one wave per tile, each wave with its own running maximum, sum and output; the
+// four waves meet in LDS at the end, the pieces of a split key range in a second kernel.
+//
+// S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4: K's codes are the operand as they lie in the cache, the page's
+// e8m0 scale rides in the instruction's scale operand, and q is the sum of two e4m3 terms with scales of their own (hi:
+// rounded at the row's block exponent; lo: the remainder times 16, which has at most four significant bits, so the sum is
+// exact down to 2^-22 of the row's largest element).  Two fp8 products of 128 elements take the matrix pipe as long as
+// the four bf16 products that expanding K would need, and K is never expanded.
+// O^T += V^T P^T on v_mfma_f32_16x16x32_f16: V's codes are exact in fp16, and the weights get fp16's eleven bits
+// instead of bf16's eight.  fp16's range is kept safe by the weight's unit: with e_v the exponent of the block's scale,
+//   w = exp2(s c + e_v + 14 - m),  m = running maximum of s c + e_v   (c = softmax_scale log2 e),
+// lies in (0, 2^14], multiplies the raw codes, and the row sum adds 2^-e_v w.  |e_v| <= 48 bounds what two blocks can be
+// apart to 2^96: a weight, or the factor that joins two partial sums, leaves fp32's normal range (2^-126) only for
+// tokens whose share of the softmax is below 2^-30.
+// Lane (n = lane % 16, g = lane / 16) of S^T holds query n, keys 4g .. 4g + 3 of a 16-key half: packed to fp16, the two
+// halves of a tile are the B operand of the second product as they stand.
+// A masked tile may hold NaN codes of tokens that some rows do not see: 0 * NaN must not reach those rows, so such a
+// tile takes V with the NaN replaced by 0 and adds NaN to the rows that do see it (a second product over indicators).
+#include "kv_internal.h"
+
+namespace dsx {
+namespace {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTileKeys = 32;
+constexpr float kHeadroom = 14.f;  // log2 of the largest fp16 weight
+
+struct AttnArgs {
+  dsx_kv_cache c;
+  dsx_kv_batch n;
+  dsx_kv_attn_params p;
+  int group;       // query heads per cache head
+  int page_shift;
+  int nqb;         // query blocks per (sequence, cache head)
+  int splits;      // pieces of the key range
+  float* part_o;   // (units * splits, 16 NQ, 128) fp32
+  float* part_ml;  // (units * splits, 16 NQ, 2)
+};
+
+__device__ __forceinline__ float quad_max(float v) {  // over the four lanes n, n + 16, n + 32, n + 48
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float m = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const f16x2 v = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// q row -> two e4m3 terms and their e8m0 scales.  x: the lane's 32 elements; the four lanes of a row share the exponent.
+struct QFrag {
+  i32x8 hi, lo;
+  int s_hi, s_lo;
+};
+__device__ __forceinline__ void split_q(const float (&x)[32], QFrag& f) {
+  float amax = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    amax = fmaxf(amax, fabsf(x[j]));
+    odd |= !(fabsf(x[j]) < INFINITY);
+  }
+  amax = quad_max(odd ? INFINITY : amax);
+  const uint32_t bits = __float_as_uint(amax);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = max(e, -110);
+  const bool bad = !(amax < INFINITY);
+  if (bad) e = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    float y[4], r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : ldexpf(x[4 * w + j], -e);
+    const uint32_t hi = pack_e4m3x4_inrange(y[0], y[1], y[2], y[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = 16.f * (y[j] - e4m3_bits_to_f32((hi >> (8 * j)) & 0xffu));
+    f.hi[w] = (int)hi;
+    f.lo[w] = (int)pack_e4m3x4_inrange(r[0], r[1], r[2], r[3]);
+  }
+  f.s_hi = bad ? 255 : 127 + e;
+  f.s_lo = bad ? 255 : 127 + e - 4;
+}
+
+// A tile's codes in flight.  K: row n of each 16-key half, elements 16g .. +15 and 64 + 16g .. +15.  V: tokens 4g + t,
+// elements 8n .. 8n + 7.
+struct TileRegs {
+  u32x4 k[2][2];
+  u32x2 v[2][4];
+};
+
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // 0x80 in every byte that holds e4m3's NaN
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+template <int NQ>  // 16-row columns of query rows
+__global__ __launch_bounds__(256) void kv_stream_kernel(AttnArgs a) {
+  const dsx_kv_cache& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t u = blockIdx.x;
+  const int split = (int)(u % a.splits);
+  u /= a.splits;
+  const int64_t unit = u;
+  const int qb = (int)(u % a.nqb);
+  u /= a.nqb;
+  const int h = (int)(u % c.heads), b = (int)(u / c.heads);
+  __shared__ float sm_o[4][16][kKvDim + 4];
+  __shared__ float sm_m[4][16], sm_l[4][16];
+
+  const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
+  const int packed = s.rows * a.group;
+  const int pr0 = qb * 16 * NQ;
+  if (pr0 >= packed) return;
+
+  // ---- the rows of this block and the keys any of them sees
+  const int row_lo = pr0 / a.group, row_hi = min(pr0 + 16 * NQ, packed) - 1;
+  int lo_first, hi_first, lo_last, hi_last;
+  kv_row_span(s.kv, s.rows, row_lo, a.p.causal, a.p.window, lo_first, hi_first);
+  kv_row_span(s.kv, s.rows, row_hi / a.group, a.p.causal, a.p.window, lo_last, hi_last);
+  const int tile_first = lo_first / kTileKeys;
+  const int tile_end = (hi_last + kTileKeys - 1) / kTileKeys;
+  const int per = (max(tile_end - tile_first, 0) + a.splits - 1) / a.splits;
+  const int t_begin = tile_first + split * per;
+  const int t_end = min(t_begin + per, tile_end);
+
+  // ---- q, split into its two terms
+  QFrag qf[NQ];
+  int my_lo[NQ], my_hi[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int pr = min(pr0 + q * 16 + n16, packed - 1);
+    const int row = pr / a.group, hh = h * a.group + pr % a.group;
+    kv_row_span(s.kv, s.rows, row, a.p.causal, a.p.window, my_lo[q], my_hi[q]);
+    const uint16_t* src = (const uint16_t*)a.p.q + (int64_t)(s.row0 + row) * a.p.q_sr + hh * a.p.q_sh + 16 * g4;
+    float x[32];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 64 * half + 8 * w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[16 * half + 8 * w + 2 * j] = bf16_lo(raw[j]);
+          x[16 * half + 8 * w + 2 * j + 1] = bf16_hi(raw[j]);
+        }
+      }
+    split_q(x, qf[q]);
+  }
+
+  f32x4 o[NQ][8];  // o[q][i][r]: query n of column q, element 32g + 8r + i
+  float m_run[NQ], l_run[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    m_run[q] = -INFINITY;
+    l_run[q] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float cs = a.p.softmax_scale * kLog2e;
+
+  const uint8_t* kbase = (const uint8_t*)c.k + (int64_t)h * c.k_sh;
+  const uint8_t* vbase = (const uint8_t*)c.v + (int64_t)h * c.v_sh;
+  const int koff = n16 * kKvDim + 16 * g4, voff = 4 * g4 * kKvDim + 8 * n16;
+  const int page_mask = c.page_size - 1;
+
+  // Page numbers and scales of the wave's next 64 tiles, one tile per lane: two dependent loads per 64 tiles instead
+  // of two per tile.  scales: k of the halves in bytes 0, 1, v in bytes 2, 3.
+  int pg[2];
+  uint32_t sc_all = 0;
+  const int tiles = t_end > t_begin + wave ? (t_end - t_begin - wave + 3) / 4 : 0;  // this wave's
+  auto preload = [&](int i0) {
+    const int t = t_begin + wave + 4 * (i0 + lane);
+    sc_all = 0x7f7f7f7fu;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int key = t * kTileKeys + 16 * hf;
+      pg[hf] = 0;
+      if (t < t_end && key < hi_last) {
+        const int id = a.n.page_table[b * a.n.table_sb + (key >> a.page_shift)];
+        const bool bad = id < 0 || id >= c.pages;
+        pg[hf] = bad ? 0 : id;
+        uint32_t ks = ((const uint8_t*)c.k_scale)[pg[hf] * c.ks_sp + h];
+        const uint32_t vs = ((const uint8_t*)c.v_scale)[pg[hf] * c.vs_sp + h];
+        if (bad || vs == 255) ks = 255;  // NaN scores for every row that sees the block
+        sc_all = (sc_all & ~(0xff00ffu << (8 * hf))) | (ks << (8 * hf)) | (vs << (16 + 8 * hf));
+      }
+    }
+  };
+  auto load_tile = [&](int i, TileRegs& r) -> uint32_t {  // the wave's i-th tile; returns its scales
+    if ((i & 63) == 0) preload(i);
+    const int key = (t_begin + wave + 4 * i) * kTileKeys;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int64_t page = __builtin_amdgcn_readlane(pg[hf], i & 63);
+      const int tok = (key + 16 * hf) & page_mask;
+      const uint8_t* kp = kbase + page * c.k_sp + tok * kKvDim;
+      const uint8_t* vp = vbase + page * c.v_sp + tok * kKvDim;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) r.k[hf][w] = *reinterpret_cast<const u32x4*>(kp + koff + 64 * w);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) r.v[hf][t] = *reinterpret_cast<const u32x2*>(vp + voff + t * kKvDim);
+    }
+    return (uint32_t)__builtin_amdgcn_readlane((int)sc_all, i & 63);
+  };
+
+  auto compute = [&](int i, TileRegs& r, uint32_t sc) {
+    const int key0 = (t_begin + wave + 4 * i) * kTileKeys;
+    f32x4 st[2][NQ];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const i32x8 kf = {(int)r.k[hf][0][0], (int)r.k[hf][0][1], (int)r.k[hf][0][2], (int)r.k[hf][0][3],
+                        (int)r.k[hf][1][0], (int)r.k[hf][1][1], (int)r.k[hf][1][2], (int)r.k[hf][1][3]};
+      const int ks = (int)((sc >> (8 * hf)) & 0xffu);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].lo, z, 0, 0, 0, ks, 0, qf[q].s_lo);
+        st[hf][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].hi, z, 0, 0, 0, ks, 0, qf[q].s_hi);
+      }
+    }
+    // boundary tile: some row of the block does not see some key of it
+    const bool masked = key0 < lo_last || key0 + kTileKeys > hi_first;
+    bool has_nan = false;
+    if (masked) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * hf + 4 * g4 + e;
+            if (key < my_lo[q] || key >= my_hi[q]) st[hf][q][e] = -INFINITY;
+          }
+        uint32_t any = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int key = key0 + 16 * hf + 4 * g4 + t;
+          if (key < lo_first || key >= hi_last) r.v[hf][t] = u32x2{0u, 0u};  // seen by no row: whatever lies there
+          any |= nan_bytes(r.v[hf][t][0]) | nan_bytes(r.v[hf][t][1]);
+        }
+        has_nan |= __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      }
+    }
+    const float ev[2] = {(float)((int)((sc >> 16) & 0xffu) - 127), (float)((int)(sc >> 24) - 127)};
+    const float inv_v[2] = {__uint_as_float((254u - ((sc >> 16) & 0xffu)) << 23), __uint_as_float((254u - (sc >> 24)) << 23)};
+    f16x8 pf[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      float mx[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const f32x4& v = st[hf][q];
+        mx[hf] = __builtin_fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), cs, ev[hf]);
+      }
+      const float top = quad_max(fmaxf(mx[0], mx[1]));
+      if (__builtin_amdgcn_ballot_w64(top > m_run[q]) != 0) {
+        const float m_new = fmaxf(m_run[q], top);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[q] - m_new);
+        m_run[q] = m_new;
+        l_run[q] *= alpha;
+#pragma unroll
+        for (int i2 = 0; i2 < 8; ++i2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[q][i2][e] *= alpha;
+      }
+      const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
+      u32x4 pw;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float off = ev[hf] + kHeadroom - ref;
+        float w[4], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[hf][q][e], cs, off));
+          sum += w[e];
+        }
+        l_run[q] = __builtin_fmaf(sum, inv_v[hf], l_run[q]);
+        pw[2 * hf] = pack_f16x2(w[0], w[1]);
+        pw[2 * hf + 1] = pack_f16x2(w[2], w[3]);
+      }
+      pf[q] = __builtin_bit_cast(f16x8, pw);
+    }
+    if (__builtin_expect(has_nan, 0)) {
+      f16x8 seen[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key0 + 16 * (e >> 2) + 4 * g4 + (e & 3);
+          seen[q][e] = key >= my_lo[q] && key < my_hi[q] ? (_Float16)1.f : (_Float16)0.f;
+        }
+#pragma unroll
+      for (int i2 = 0; i2 < 8; ++i2) {
+        f16x8 flag;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          flag[e] = (nan_bytes(r.v[e >> 2][e & 3][i2 >> 2]) >> (8 * (i2 & 3))) & 0x80u ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(flag, seen[q], z, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hit[e] > 0.f) o[q][i2][e] = NAN;
+        }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t bad = nan_bytes(r.v[hf][t][w]);
+            r.v[hf][t][w] &= ~((bad >> 7) * 0xffu);
+          }
+    }
+    // V^T: row n of M-tile 4w + e is element 8n + 4w + e.  Byte pairs of two tokens come together with one permute, and
+    // the converter takes either half of it.
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      uint32_t pr[2][2][2];  // [half][token pair][elements 01 | 23]
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          pr[hf][t][0] = __builtin_amdgcn_perm(r.v[hf][2 * t + 1][w], r.v[hf][2 * t][w], 0x05010400u);
+          pr[hf][t][1] = __builtin_amdgcn_perm(r.v[hf][2 * t + 1][w], r.v[hf][2 * t][w], 0x07030602u);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f16x2 d[4];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            d[2 * hf + t] = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(pr[hf][t][e >> 1], 1.0f, true)
+                                  : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(pr[hf][t][e >> 1], 1.0f, false);
+        const f16x8 vf = {d[0][0], d[0][1], d[1][0], d[1][1], d[2][0], d[2][1], d[3][0], d[3][1]};
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          o[q][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q], o[q][4 * w + e], 0, 0, 0);
+      }
+    }
+  };
+
+  TileRegs ra, rb;
+  uint32_t sa = 0, sb = 0;
+  if (tiles > 0) sa = load_tile(0, ra);
+  for (int i = 0; i < tiles; i += 2) {
+    if (i + 1 < tiles) sb = load_tile(i + 1, rb);
+    compute(i, ra, sa);
+    if (i + 1 < tiles) {
+      if (i + 2 < tiles) sa = load_tile(i + 2, ra);
+      compute(i + 1, rb, sb);
+    }
+  }
+
+  // ---- the four waves' results join in LDS, one 16-row column at a time: thread (row, 8 elements)
+  const int row16 = tid >> 4, d0 = (tid & 15) * 8;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    if (q) __syncthreads();
+    const float l = quad_sum(l_run[q]);
+    if (g4 == 0) {
+      sm_m[wave][n16] = m_run[q];
+      sm_l[wave][n16] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        *reinterpret_cast<f32x4*>(&sm_o[wave][n16][32 * g4 + 8 * r + i]) =
+            f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
+    __syncthreads();
+    float m = fmaxf(fmaxf(sm_m[0][row16], sm_m[1][row16]), fmaxf(sm_m[2][row16], sm_m[3][row16]));
+    float lt = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = sm_m[w][row16] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(sm_m[w][row16] - m);
+      lt = __builtin_fmaf(sm_l[w][row16], f, lt);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(sm_o[w][row16][d0 + e], f, acc[e]);
+    }
+    const int pr = pr0 + q * 16 + row16;
+    if (a.splits > 1) {
+      const int64_t at = (unit * a.splits + split) * (16 * NQ) + q * 16 + row16;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(a.part_o + at * kKvDim + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+      if (d0 == 0) {
+        a.part_ml[2 * at] = m;
+        a.part_ml[2 * at + 1] = lt;
+      }
+    } else if (pr < packed) {
+      const float inv = s.ok ? (lt == 0.f ? 0.f : 1.f / lt) : NAN;
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      const int row = pr / a.group, hh = h * a.group + pr % a.group;
+      *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+    }
+  }
+}
+
+// Joins the pieces of split key ranges: 16 lanes per packed query row, 8 elements per lane.
+template <int NQ>
+__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
+  const dsx_kv_cache& c = a.c;
+  const int row16 = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  int64_t u = blockIdx.x;
+  const int q = (int)(u % NQ);
+  u /= NQ;
+  const int64_t unit = u;
+  const int qb = (int)(u % a.nqb);
+  u /= a.nqb;
+  const int h = (int)(u % c.heads), b = (int)(u / c.heads);
+  const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
+  const int pr = qb * 16 * NQ + q * 16 + row16;
+  if (pr >= s.rows * a.group) return;
+  const int64_t at = unit * a.splits * (16 * NQ) + q * 16 + row16;
+  float m = -INFINITY;
+  for (int t = 0; t < a.splits; ++t) m = fmaxf(m, a.part_ml[2 * (at + (int64_t)t * 16 * NQ)]);
+  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < a.splits; ++t) {
+    const int64_t r = at + (int64_t)t * 16 * NQ;
+    const float mt = a.part_ml[2 * r];
+    const float f = mt == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mt - m);
+    l = __builtin_fmaf(a.part_ml[2 * r + 1], f, l);
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + r * kKvDim + d0 + e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[e + j] = __builtin_fmaf(v[j], f, acc[e + j]);
+    }
+  }
+  const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  const int row = pr / a.group, hh = h * a.group + pr % a.group;
+  *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+}
+
+struct Plan {
+  int nq, nqb, splits;
+  int64_t units, ws_bytes;
+};
+
+int check(const dsx_kv_cache* c, const dsx_kv_batch* n, const dsx_kv_attn_params* p) {
+  if (!p) return DSX_ENULL;
+  const int rc = kv_check_cache(c, n, p->total_rows);
+  if (rc != DSX_OK) return rc;
+  if (p->heads_q < 1 || p->heads_q % c->heads || p->window < 0) return DSX_EBADSHAPE;
+  if (!(p->softmax_scale > 0.f) || !(p->softmax_scale < INFINITY)) return DSX_EBADSHAPE;
+  if ((int64_t)n->max_rows * (p->heads_q / c->heads) > (1 << 30)) return DSX_EBADSHAPE;
+  return DSX_OK;
+}
+
+Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_params& p) {
+  Plan r{};
+  const int64_t rows = n.max_rows < p.total_rows ? n.max_rows : p.total_rows;
+  const int64_t packed = rows * (p.heads_q / c.heads);
+  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : 4;
+  r.nqb = (int)((packed + 16 * r.nq - 1) / (16 * r.nq));
+  r.units = (int64_t)n.batch * c.heads * r.nqb;
+  const int64_t span = p.window > 0 && p.window + rows < n.max_kv_len ? p.window + rows : n.max_kv_len;
+  const int64_t most = (span + 255) / 256;
+  const int64_t want = r.units > 0 ? (1024 + r.units - 1) / r.units : 1;
+  r.splits = (int)(want < most ? want : most);
+  if (r.splits < 1) r.splits = 1;
+  r.ws_bytes = r.splits > 1 ? r.units * r.splits * 16 * r.nq * (kKvDim + 2) * 4 : 0;
+  return r;
+}
+
+template <int NQ>
+void launch(const AttnArgs& a, int64_t units, hipStream_t st) {
+  kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(256), 0, st>>>(a);
+  if (a.splits > 1) kv_join_kernel<NQ><<<dim3((unsigned)(units * NQ)), dim3(256), 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace dsx
+
+extern "C" int64_t dsx_kv_attn_workspace_bytes(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
+                                                const dsx_kv_attn_params* p) {
+  using namespace dsx;
+  if (check(cache, batch, p) != DSX_OK) return 0;
+  return make_plan(*cache, *batch, *p).ws_bytes;
+}
+
+extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
+                                                const dsx_kv_attn_params* p, void* stream) {
+  using namespace dsx;
+  const int rc = check(cache, batch, p);
+  if (rc != DSX_OK) return rc;
+  const dsx_kv_cache& c = *cache;
+  const dsx_kv_batch& n = *batch;
+  if (!p->q || !p->out) return DSX_ENULL;
+  if ((((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->workspace) & 15) || p->q_sr % 8 || p->q_sh % 8 ||
+      p->o_sr % 8 || p->o_sh % 8)
+    return DSX_EALIGN;
+  if (n.max_rows == 0 || p->total_rows == 0) return DSX_OK;
+  Plan plan = make_plan(c, n, *p);
+  if (plan.splits > 1) {
+    if (!p->workspace)
+      plan.splits = 1;
+    else if (p->workspace_bytes < plan.ws_bytes)
+      return DSX_EWORKSPACE;
+  }
+  if (plan.units * plan.splits >= (1ll << 31) || plan.units * plan.nq >= (1ll << 31)) return DSX_EBADSHAPE;
+  AttnArgs a{};
+  a.c = c;
+  a.n = n;
+  a.p = *p;
+  a.group = p->heads_q / c.heads;
+  a.page_shift = __builtin_ctz((unsigned)c.page_size);
+  a.nqb = plan.nqb;
+  a.splits = plan.splits;
+  if (plan.splits > 1) {
+    a.part_o = (float*)p->workspace;
+    a.part_ml = a.part_o + plan.units * plan.splits * 16 * plan.nq * kKvDim;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (plan.nq == 1)
+    launch<1>(a, plan.units, st);
+  else if (plan.nq == 2)
+    launch<2>(a, plan.units, st);
+  else
+    launch<4>(a, plan.units, st);
+  return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;
+}

@@ -1,0 +1,42 @@
+// What the paged 8-bit key/value cache's kernels share: the cache's addressing with its bounds, and the block scale.
+// Everything here also compiles for the host (dsx_kv_plan_check walks the same functions).
+#pragma once
+#include "common.h"
+
+namespace dsx {
+
+constexpr int kKvDim = 128;
+constexpr int kScaleMin = -48, kScaleMax = 48;  // exponents a block scale takes (why: kv_attn.hip)
+
+// One sequence of a packed batch.  The lengths live on the device and nothing on the host has seen them, so every
+// kernel checks them against the bounds the host has checked the buffers with: `ok` false means that nothing of the
+// sequence may be touched but its output rows, and `rows` is 0 when not even those can be named.
+struct KvSeq {
+  int row0, rows, kv;
+  bool ok;
+};
+__host__ __device__ inline KvSeq kv_seq(const dsx_kv_batch& n, int b, int64_t total_rows) {
+  const int r0 = n.row_start[b], r1 = n.row_start[b + 1], kv = n.kv_len[b];
+  if (r0 < 0 || r1 < r0 || r1 > total_rows) return {0, 0, 0, false};
+  const bool ok = r1 - r0 <= n.max_rows && kv >= 0 && kv <= n.max_kv_len;
+  return {r0, r1 - r0 <= n.max_rows ? r1 - r0 : n.max_rows, ok ? kv : 0, ok};
+}
+
+// Tokens [begin, end) that row i of a sequence sees.
+__host__ __device__ inline void kv_row_span(int kv, int rows, int i, int causal, int window, int& begin, int& end) {
+  end = causal ? kv - rows + i + 1 : kv;
+  if (end < 0) end = 0;
+  begin = window > 0 && end > window ? end - window : 0;
+}
+
+// Smallest e in [kScaleMin, kScaleMax] with amax <= 448 * 2^e (448 = 1.75 * 2^8); amax finite, >= 0.
+__host__ __device__ inline int kv_block_exponent(uint32_t amax_bits) {
+  int e = (int)(amax_bits >> 23) - 127 - 8;
+  if ((amax_bits & 0x7fffffu) > 0x600000u) ++e;
+  return e < kScaleMin ? kScaleMin : e > kScaleMax ? kScaleMax : e;
+}
+
+// Host checks of the part both calls share.
+int kv_check_cache(const dsx_kv_cache* c, const dsx_kv_batch* n, int64_t total_rows);
+
+}  // namespace dsx

@@ -4,12 +4,15 @@ PyTorch is used for device memory and the current stream only; every function be
 hand-written gfx950 kernels from libdsx.so on ``torch.cuda.current_stream()`` and raises if the
 library is missing or the tensors are not on a GPU.
 """
+import contextlib
+import ctypes
 import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from .kv_cache import HEAD_DIM, KVCache, KVPlan
 
 FP8 = torch.float8_e4m3fn
 _BF16 = torch.bfloat16
@@ -636,4 +639,125 @@ def flow_match_euler_step(latents: torch.Tensor, model_outputs: torch.Tensor, dt
     rc = _lib.load().dsx_flow_match_euler_step(_ptr(a), _ptr(b), float(dt), _ptr(out), a.numel(),
                                                int(a.dtype == torch.float32), _stream())
     _lib.check(rc, "dsx_flow_match_euler_step")
+    return out
+
+
+def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None):
+    """(pointer, row stride, head stride) of a (rows, heads, 128) bf16 view."""
+    if t.dtype != _BF16 or t.dim() != 3 or t.shape[0] != rows or t.shape[2] != HEAD_DIM \
+            or (heads is not None and t.shape[1] != heads):
+        raise ValueError("%s must be bf16 (%d, %s, 128), got %s %s"
+                         % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(t.shape)))
+    sr, sh, sd = t.stride()
+    ptr = t.data_ptr()
+    if sd != 1 or sr % 8 or sh % 8 or ptr % 16:
+        raise ValueError("%s needs unit stride in the head dim, other strides in multiples of 8 and 16-byte alignment"
+                         % name)
+    return ptr, sr, sh
+
+
+def _on(device: torch.device):
+    """Makes the tensors' device the current one where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
+              k_norm_w: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              q: Optional[torch.Tensor] = None, q_norm_w: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Append packed rows to a paged 8-bit cache, and prepare their queries, in one launch.
+
+    k, v: (rows, cache.heads, 128) bf16, q: (rows, heads, 128) bf16; unit stride in the last dim, other strides in
+    multiples of 8 (slices of one packed projection are fine).  k gets RMSNorm per head (k_norm_w (128,), optional) and
+    the rotation of its position's row of ``rope`` (fp32 (B|1, >= plan.max_kv_len, 64, 2) (cos, sin), optional), q the
+    same with q_norm_w; a row's position is its token number in its sequence.  fp32 throughout, rounded once: k and v
+    to e4m3 with one power-of-two scale per (page, head) block, q to bf16.
+
+    A block that keeps earlier tokens never lowers its scale; when it has to grow, the kept codes are rounded to the new
+    one.  Infinities saturate, NaN stays NaN.  Appending the same rows at the same positions again changes nothing.
+    A page must belong to one sequence while it is appended to.  Rows of a sequence that breaks a bound of the plan are
+    not appended (``plan.check`` finds them); rows behind the last sequence are left alone, in q_out too.
+
+    Returns q prepared (``q_out`` or a new tensor; q_out may be q), or None without q."""
+    _require_cuda(k, v, q, q_out, k_norm_w, q_norm_w, rope)
+    plan._fits(cache, k.device)
+    rows = k.shape[0]
+    P = _lib.KVAppendParams(total_rows=rows, norm_eps=eps)
+    P.k, P.k_sr, P.k_sh = _kv_rows("kv_append: k", k, rows, cache.heads)
+    P.v, P.v_sr, P.v_sh = _kv_rows("kv_append: v", v, rows, cache.heads)
+    if not eps >= 0:
+        raise ValueError("kv_append: eps must not be negative")
+    keep = []
+    if q is None:
+        if q_norm_w is not None or q_out is not None:
+            raise ValueError("kv_append: q_norm_w and q_out go with q")
+    else:
+        P.q, P.q_sr, P.q_sh = _kv_rows("kv_append: q", q, rows)
+        P.heads_q = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
+        P.q_out, P.qo_sr, P.qo_sh = _kv_rows("kv_append: q_out", q_out, rows, q.shape[1])
+    for name, w in (("k_norm_w", k_norm_w), ("q_norm_w", q_norm_w)):
+        if w is not None:
+            if w.numel() != HEAD_DIM:
+                raise ValueError("kv_append: RMSNorm weights have 128 entries")
+            w = w.to(_BF16).contiguous()
+            if w.data_ptr() % 16:
+                w = w.clone()
+            keep.append(w)
+            setattr(P, name, w.data_ptr())
+    if rope is not None:
+        rope = _rope_table(rope, plan.batch, plan.max_kv_len)
+        keep.append(rope)
+        P.rope, P.rope_rows = rope.data_ptr(), rope.shape[1]
+        P.rope_sb = rope.stride(0) if rope.shape[0] > 1 else 0
+    if any(t is not None and t.device != k.device for t in (v, q, q_out, k_norm_w, q_norm_w, rope)):
+        raise ValueError("kv_append: all tensors must be on one device")
+    if rows and (P.heads_q or q is None):
+        with _on(k.device):
+            _lib.check(_lib.load().dsx_kv_append(cache._ref, plan._ref, ctypes.byref(P), _stream()), "dsx_kv_append")
+    return q_out
+
+
+def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool = True, window: int = 0,
+                 scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                 split_keys: bool = True) -> torch.Tensor:
+    """softmax(q k^T * scale) v of packed rows over the tokens their sequences have in a paged 8-bit cache.
+
+    q, out: (rows, heads, 128) bf16, heads a multiple of cache.heads (query head h reads cache head
+    h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8.
+    causal: row i of a sequence with r rows sees its first kv_len - r + i + 1 tokens; else all kv_len.  Of these only the
+    last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive.
+
+    Rows of a sequence that breaks a bound of the plan become NaN, and so do rows that see a token whose page number is
+    out of range.  Rows of ``out`` behind the last sequence are left as they are (and hold nothing meaningful in an
+    ``out`` made here).  Where units of work are few, their key ranges are split over the chip through a workspace
+    allocated here (split_keys=False: never)."""
+    _require_cuda(q, out)
+    plan._fits(cache, q.device)
+    rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    P = _lib.KVAttnParams(total_rows=rows, heads_q=heads, causal=int(bool(causal)), window=window,
+                          softmax_scale=1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    P.q, P.q_sr, P.q_sh = _kv_rows("kv_attention: q", q, rows)
+    if heads < 1 or heads % cache.heads:
+        raise ValueError("kv_attention: %d query heads for %d cache heads" % (heads, cache.heads))
+    if window < 0 or window > 0x7fffffff:
+        raise ValueError("kv_attention: window must lie in [0, 2^31)")
+    if not 0.0 < P.softmax_scale < math.inf:
+        raise ValueError("kv_attention: scale must be positive and finite")
+    if out is None:
+        out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
+    elif out.device != q.device:
+        raise ValueError("kv_attention: all tensors must be on one device")
+    P.out, P.o_sr, P.o_sh = _kv_rows("kv_attention: out", out, rows, heads)
+    if not rows:
+        return out
+    lib = _lib.load()
+    with _on(q.device):
+        p = ctypes.byref(P)
+        need = lib.dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, p) if split_keys else 0
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            P.workspace, P.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.dsx_kv_attn(cache._ref, plan._ref, p, _stream()), "dsx_kv_attn")
     return out

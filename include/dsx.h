@@ -376,6 +376,103 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
                               int is_fp32, void* stream);
 
 /*
+ * A paged key/value cache of one attention layer, held in 8 bits, and the batch that a call works on.
+ * (No counterpart in the reference, which keeps no keys or values between calls.)
+ *
+ * Codes: e4m3, element (page, head, token, d) of k at k + page*k_sp + head*k_sh + token*128 + d (v likewise).
+ * Scales: e8m0 (a byte x stands for 2^(x-127)), one per (page, head), at k_scale + page*ks_sp + head; the value that a
+ * code stands for is code * scale.  Exponents are in [-48, 48]; byte 255 makes every row that sees the block NaN.
+ *
+ * A batch is packed row-wise: rows [row_start[b], row_start[b+1]) of q, k, v and the outputs belong to sequence b, whose
+ * cache holds kv_len[b] tokens, these rows (the newest) included; token t of it lives in page
+ * page_table[b*table_sb + t / page_size].  row_start (batch+1), kv_len (batch) and page_table are int32 on the DEVICE and
+ * may change between calls, replays of a captured call included; max_rows, max_kv_len, the calls' total_rows and
+ * table_pages bound them and are what buffers and launches are sized by.  The kernels hold every value against its bound: a sequence
+ * whose lengths break one is not appended and its rows (as far as they lie in the output) leave attention as NaN; a
+ * page number outside [0, pages) is not written, and rows that see a token of it become NaN.  dsx_kv_plan_check does the
+ * same checks on the host.
+ * Rows from row_start[batch] on belong to nobody and are left as they are.
+ */
+typedef struct dsx_kv_cache {
+  void* k; void* v;
+  void* k_scale; void* v_scale;
+  int64_t k_sp, k_sh, v_sp, v_sh;    /* page and head strides of the codes, multiples of 16 */
+  int64_t ks_sp, vs_sp;              /* page strides of the scales */
+  int32_t pages, heads, page_size;   /* page_size: 16, 32, 64 or 128 tokens */
+} dsx_kv_cache;
+
+typedef struct dsx_kv_batch {
+  const int32_t* page_table; int64_t table_sb;
+  const int32_t* row_start;
+  const int32_t* kv_len;
+  int32_t batch, table_pages;        /* table_pages: columns of page_table, table_sb >= table_pages */
+  int32_t max_rows, max_kv_len;      /* max_kv_len <= table_pages * page_size; both <= 2^30 */
+} dsx_kv_batch;
+
+/*
+ * Appends a batch's rows to the cache and prepares its queries, one launch:
+ *   k: RMSNorm over the head (k_norm_w bf16 (128,), NULL = none), rotation of the pairs (2i, 2i+1) by the (cos, sin) of
+ *      table row `position` (rope NULL = none), block scale, e4m3;   v: block scale, e4m3;
+ *   q (NULL = none): RMSNorm (q_norm_w), rotation, bf16 to q_out (which may be q itself).
+ * A row's position is its token number in its sequence.  fp32 throughout, rounded once where it is stored (the row
+ * kernels dsx_rmsnorm_rope* round to bf16 in between).
+ * Block scale: with a the largest finite magnitude among the block's new tokens, e = the smallest integer in [-48, 48]
+ * with a <= 448 * 2^e.  A block that keeps earlier tokens takes max(e, its present exponent), and its kept codes are
+ * rounded to the new scale when that is larger; they are not touched otherwise.  Values beyond the range saturate
+ * (infinities too), NaN stays NaN.  Writing the same rows to the same positions again gives the same cache.
+ * A page must not be appended to by two sequences of a batch, nor while another stream reads it.
+ * k, v: (total_rows, heads, 128) bf16, q and q_out: (total_rows, heads_q, 128), by row and head strides (multiples of
+ * 8, 16-byte aligned).  rope: fp32 (cos, sin) rows of 128 floats, rope_rows >= max_kv_len per sequence, rope_sb 0 (one
+ * table) or >= rope_rows*128.
+ */
+typedef struct dsx_kv_append_params {
+  const void* k; int64_t k_sr, k_sh;
+  const void* v; int64_t v_sr, v_sh;
+  const void* q; int64_t q_sr, q_sh;
+  void* q_out; int64_t qo_sr, qo_sh;
+  const void* k_norm_w; const void* q_norm_w;
+  const float* rope; int64_t rope_sb, rope_rows;
+  int64_t total_rows;                /* rows that k, v, q and q_out have */
+  float norm_eps;
+  int32_t heads_q;
+} dsx_kv_append_params;
+int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const dsx_kv_append_params* p, void* stream);
+
+/*
+ * Attention of a batch's rows over its cached tokens: out = softmax(softmax_scale * q k^T) v, where row i of a sequence
+ * with `rows` rows sees the tokens [0, end), end = kv_len - rows + i + 1 with `causal`, kv_len without, and of those the
+ * last `window` when window > 0.  A row that sees nothing gives zeros (causal rows with negative positions; kv_len 0).
+ * Query head h reads cache head h / (heads_q / heads); heads_q is a multiple of heads.
+ * Softmax and sums in fp32.  q is used as the exact sum of two scaled e4m3 terms (each element to 2^-22 of its row's
+ * largest), the weights enter the second product as fp16.  A q row with a non-finite element gives NaN.
+ * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned).
+ * workspace: dsx_kv_attn_workspace_bytes(...) bytes, 16-byte aligned, lets the key range be split over the compute units
+ * and the pieces be joined by a second launch; NULL: never split.  Calls that share a workspace must not overlap.
+ */
+typedef struct dsx_kv_attn_params {
+  const void* q; int64_t q_sr, q_sh;
+  void* out; int64_t o_sr, o_sh;
+  int64_t total_rows;                /* rows that q and out have */
+  float softmax_scale;               /* > 0 */
+  int32_t heads_q, causal, window;
+  void* workspace; int64_t workspace_bytes;
+} dsx_kv_attn_params;
+int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const dsx_kv_attn_params* p, void* stream);
+
+/* Workspace with which dsx_kv_attn(cache, batch, p) splits as it likes; 0: it would not.  Launches nothing. */
+int64_t dsx_kv_attn_workspace_bytes(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
+                                    const dsx_kv_attn_params* p);
+
+/*
+ * The kernels' own checks on HOST copies of the three arrays (batch->row_start, kv_len and page_table point to host
+ * memory here) against `pages` pages and `total_rows` rows: DSX_OK, or DSX_EBADSHAPE with the number of the first
+ * sequence that breaks a bound in *bad_sequence.  for_append: also that kv_len >= rows, and that no page that is
+ * appended to is listed twice.  Touches no device.
+ */
+int dsx_kv_plan_check(const dsx_kv_batch* batch, int32_t pages, int32_t page_size, int64_t total_rows, int for_append,
+                      int32_t* bad_sequence);
+
+/*
  * Diagnostic, no counterpart in the reference: the on-box microbenchmark behind the roofline denominators.
  * Launches `workgroups` workgroups of four wavefronts that each run `iters` rounds of MFMAs on independent
  * accumulators (kind 0: v_mfma_f32_32x32x16_bf16, kind 1: v_mfma_f32_32x32x64 on e4m3 operands, four per round;
