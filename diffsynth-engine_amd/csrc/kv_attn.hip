@@ -62,6 +62,12 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
+// The factor that brings a partial sum with reference `m` to the reference `to` >= m.  A part that saw no token has
+// reference -inf and sums of 0 (or NaN, which must survive): 0 unless nothing else saw one either.
+__device__ __forceinline__ float join_factor(float m, float to) {
+  return m == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - to);
+}
+
 // q row -> two e4m3 terms and their e8m0 scales.  x: the lane's 32 elements; the four lanes of a row share the exponent.
 struct QFrag {
   i32x8 hi, lo;
@@ -81,16 +87,17 @@ __device__ __forceinline__ void split_q(const float (&x)[32], QFrag& f) {
   e = max(e, -110);
   const bool bad = !(amax < INFINITY);
   if (bad) e = 0;
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, a normal number for e in [-110, 120]
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
-    float y[4], r[4];
+    float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : ldexpf(x[4 * w + j], -e);
+    for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : x[4 * w + j] * down;
     const uint32_t hi = pack_e4m3x4_inrange(y[0], y[1], y[2], y[3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = 16.f * (y[j] - e4m3_bits_to_f32((hi >> (8 * j)) & 0xffu));
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
     f.hi[w] = (int)hi;
-    f.lo[w] = (int)pack_e4m3x4_inrange(r[0], r[1], r[2], r[3]);
+    f.lo[w] = (int)pack_e4m3x4_inrange(16.f * (y[0] - a[0]), 16.f * (y[1] - a[1]), 16.f * (y[2] - b[0]),
+                                       16.f * (y[3] - b[1]));
   }
   f.s_hi = bad ? 255 : 127 + e;
   f.s_lo = bad ? 255 : 127 + e - 4;
@@ -108,7 +115,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // 0x80 in every by
 }
 
 template <int NQ>  // 16-row columns of query rows
-__global__ __launch_bounds__(256) void kv_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -391,7 +398,7 @@ __global__ __launch_bounds__(256) void kv_stream_kernel(AttnArgs a) {
     float lt = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = sm_m[w][row16] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(sm_m[w][row16] - m);
+      const float f = join_factor(sm_m[w][row16], m);
       lt = __builtin_fmaf(sm_l[w][row16], f, lt);
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(sm_o[w][row16][d0 + e], f, acc[e]);
@@ -417,43 +424,64 @@ __global__ __launch_bounds__(256) void kv_stream_kernel(AttnArgs a) {
   }
 }
 
-// Joins the pieces of split key ranges: 16 lanes per packed query row, 8 elements per lane.
+// Joins the pieces of a split key range: one workgroup per packed query row, 16 lanes x 8 elements for each of 16 pieces
+// at a time, then the 16 partial joins in LDS (in a fixed order).  The pieces of a row are read at once: with all of them
+// behind one another in a lane the join of 26 pieces took 25 us.
 template <int NQ>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
-  const int row16 = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
+  __shared__ float sm_o[16][kKvDim + 4];
+  __shared__ float sm_m[16], sm_l[16];
   int64_t u = blockIdx.x;
-  const int q = (int)(u % NQ);
-  u /= NQ;
+  const int r16 = (int)(u % (16 * NQ));
+  u /= 16 * NQ;
   const int64_t unit = u;
   const int qb = (int)(u % a.nqb);
   u /= a.nqb;
   const int h = (int)(u % c.heads), b = (int)(u / c.heads);
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
-  const int pr = qb * 16 * NQ + q * 16 + row16;
+  const int pr = qb * 16 * NQ + r16;
   if (pr >= s.rows * a.group) return;
-  const int64_t at = unit * a.splits * (16 * NQ) + q * 16 + row16;
-  float m = -INFINITY;
-  for (int t = 0; t < a.splits; ++t) m = fmaxf(m, a.part_ml[2 * (at + (int64_t)t * 16 * NQ)]);
-  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int t = 0; t < a.splits; ++t) {
-    const int64_t r = at + (int64_t)t * 16 * NQ;
-    const float mt = a.part_ml[2 * r];
-    const float f = mt == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mt - m);
-    l = __builtin_fmaf(a.part_ml[2 * r + 1], f, l);
+  float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int t = grp; t < a.splits; t += 16) {
+    const int64_t at = (unit * a.splits + t) * (16 * NQ) + r16;
+    const float mt = a.part_ml[2 * at], lt = a.part_ml[2 * at + 1];
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0);
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0 + 4);
+    const float mn = fmaxf(m, mt);
+    const float fo = join_factor(m, mn), fn = join_factor(mt, mn);
+    m = mn;
+    l = l * fo + lt * fn;
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + r * kKvDim + d0 + e);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[e + j] = __builtin_fmaf(v[j], f, acc[e + j]);
+    for (int e = 0; e < 4; ++e) {
+      acc[e] = acc[e] * fo + lo[e] * fn;
+      acc[4 + e] = acc[4 + e] * fo + hi[e] * fn;
     }
   }
+  *reinterpret_cast<f32x4*>(&sm_o[grp][d0]) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+  *reinterpret_cast<f32x4*>(&sm_o[grp][d0 + 4]) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+  if (d0 == 0) {
+    sm_m[grp] = m;
+    sm_l[grp] = l;
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  const int groups = min(a.splits, 16);
+  m = -INFINITY;
+  for (int g = 0; g < groups; ++g) m = fmaxf(m, sm_m[g]);
+  float o0 = 0.f, o1 = 0.f;
+  l = 0.f;
+  for (int g = 0; g < groups; ++g) {
+    const float f = join_factor(sm_m[g], m);
+    l = __builtin_fmaf(sm_l[g], f, l);
+    o0 = __builtin_fmaf(sm_o[g][2 * tid], f, o0);
+    o1 = __builtin_fmaf(sm_o[g][2 * tid + 1], f, o1);
+  }
   const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
-  u32x4 w;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   const int row = pr / a.group, hh = h * a.group + pr % a.group;
-  *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+  *reinterpret_cast<uint32_t*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + 2 * tid) =
+      pack_bf16x2(o0 * inv, o1 * inv);
 }
 
 struct Plan {
@@ -490,7 +518,7 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
 template <int NQ>
 void launch(const AttnArgs& a, int64_t units, hipStream_t st) {
   kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(256), 0, st>>>(a);
-  if (a.splits > 1) kv_join_kernel<NQ><<<dim3((unsigned)(units * NQ)), dim3(256), 0, st>>>(a);
+  if (a.splits > 1) kv_join_kernel<NQ><<<dim3((unsigned)(units * 16 * NQ)), dim3(256), 0, st>>>(a);
 }
 
 }  // namespace
@@ -522,7 +550,7 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
     else if (p->workspace_bytes < plan.ws_bytes)
       return DSX_EWORKSPACE;
   }
-  if (plan.units * plan.splits >= (1ll << 31) || plan.units * plan.nq >= (1ll << 31)) return DSX_EBADSHAPE;
+  if (plan.units * plan.splits >= (1ll << 31) || plan.units * plan.nq * 16 >= (1ll << 31)) return DSX_EBADSHAPE;
   AttnArgs a{};
   a.c = c;
   a.n = n;
