@@ -20,88 +20,13 @@
 // halves of a tile are the B operand of the second product as they stand.
 // A masked tile may hold NaN codes of tokens that some rows do not see: 0 * NaN must not reach those rows, so such a
 // tile takes V with the NaN replaced by 0 and adds NaN to the rows that do see it (a second product over indicators).
-#include "kv_internal.h"
+#include "kv_attn_internal.h"
 
 namespace dsx {
 namespace {
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileKeys = 32;
 constexpr float kHeadroom = 14.f;  // log2 of the largest fp16 weight
-
-struct AttnArgs {
-  dsx_kv_cache c;
-  dsx_kv_batch n;
-  dsx_kv_attn_params p;
-  int group;       // query heads per cache head
-  int page_shift;
-  int nqb;         // query blocks per (sequence, cache head)
-  int splits;      // pieces of the key range
-  float* part_o;   // (units * splits, 16 NQ, 128) fp32
-  float* part_ml;  // (units * splits, 16 NQ, 2)
-};
-
-__device__ __forceinline__ float quad_max(float v) {  // over the four lanes n, n + 16, n + 32, n + 48
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  const float m = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const f16x2 v = {(_Float16)lo, (_Float16)hi};
-  return __builtin_bit_cast(uint32_t, v);
-}
-
-// The factor that brings a partial sum with reference `m` to the reference `to` >= m.  A part that saw no token has
-// reference -inf and sums of 0 (or NaN, which must survive): 0 unless nothing else saw one either.
-__device__ __forceinline__ float join_factor(float m, float to) {
-  return m == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - to);
-}
-
-// q row -> two e4m3 terms and their e8m0 scales.  x: the lane's 32 elements; the four lanes of a row share the exponent.
-struct QFrag {
-  i32x8 hi, lo;
-  int s_hi, s_lo;
-};
-__device__ __forceinline__ void split_q(const float (&x)[32], QFrag& f) {
-  float amax = 0.f;
-  bool odd = false;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    amax = fmaxf(amax, fabsf(x[j]));
-    odd |= !(fabsf(x[j]) < INFINITY);
-  }
-  amax = quad_max(odd ? INFINITY : amax);
-  const uint32_t bits = __float_as_uint(amax);
-  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  e = max(e, -110);
-  const bool bad = !(amax < INFINITY);
-  if (bad) e = 0;
-  const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, a normal number for e in [-110, 120]
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    float y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : x[4 * w + j] * down;
-    const uint32_t hi = pack_e4m3x4_inrange(y[0], y[1], y[2], y[3]);
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
-    f.hi[w] = (int)hi;
-    f.lo[w] = (int)pack_e4m3x4_inrange(16.f * (y[0] - a[0]), 16.f * (y[1] - a[1]), 16.f * (y[2] - b[0]),
-                                       16.f * (y[3] - b[1]));
-  }
-  f.s_hi = bad ? 255 : 127 + e;
-  f.s_lo = bad ? 255 : 127 + e - 4;
-}
 
 // A tile's codes in flight.  K: row n of each 16-key half, elements 16g .. +15 and 64 + 16g .. +15.  V: tokens 4g + t,
 // elements 8n .. 8n + 7.
@@ -110,22 +35,15 @@ struct TileRegs {
   u32x2 v[2][4];
 };
 
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // 0x80 in every byte that holds e4m3's NaN
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-}
-
 template <int NQ>  // 16-row columns of query rows
 __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int64_t u = blockIdx.x;
-  const int split = (int)(u % a.splits);
-  u /= a.splits;
-  const int64_t unit = u;
-  const int qb = (int)(u % a.nqb);
-  u /= a.nqb;
-  const int h = (int)(u % c.heads), b = (int)(u / c.heads);
+  const int split = (int)(blockIdx.x % a.splits);
+  const int64_t unit = blockIdx.x / a.splits;
+  int b, h, qb;
+  kv_unit(a, unit, b, h, qb);
   __shared__ float sm_o[4][16][kKvDim + 4];
   __shared__ float sm_m[4][16], sm_l[4][16];
 
@@ -150,23 +68,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
   int my_lo[NQ], my_hi[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const int pr = min(pr0 + q * 16 + n16, packed - 1);
-    const int row = pr / a.group, hh = h * a.group + pr % a.group;
-    kv_row_span(s.kv, s.rows, row, a.p.causal, a.p.window, my_lo[q], my_hi[q]);
-    const uint16_t* src = (const uint16_t*)a.p.q + (int64_t)(s.row0 + row) * a.p.q_sr + hh * a.p.q_sh + 16 * g4;
-    float x[32];
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 64 * half + 8 * w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[16 * half + 8 * w + 2 * j] = bf16_lo(raw[j]);
-          x[16 * half + 8 * w + 2 * j + 1] = bf16_hi(raw[j]);
-        }
-      }
-    split_q(x, qf[q]);
+    load_q(a, s, h, min(pr0 + q * 16 + n16, packed - 1), g4, qf[q], my_lo[q], my_hi[q]);
   }
 
   f32x4 o[NQ][8];  // o[q][i][r]: query n of column q, element 32g + 8r + i
@@ -424,28 +326,25 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
   }
 }
 
-// Joins the pieces of a split key range: one workgroup per packed query row, 16 lanes x 8 elements for each of 16 pieces
-// at a time, then the 16 partial joins in LDS (in a fixed order).  The pieces of a row are read at once: with all of them
-// behind one another in a lane the join of 26 pieces took 25 us.
-template <int NQ>
-__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
-  const dsx_kv_cache& c = a.c;
+// Joins the pieces of split key ranges.  16 lanes x 8 elements read one piece of one packed query row; the 16 such groups
+// of a workgroup take `ways` pieces of 16 / ways rows at once (ways: the number of pieces, up to a power of two and 16)
+// and meet in LDS in a fixed order.  All pieces behind one another in a lane took 25 us for 26 of them.
+__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
   const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
   __shared__ float sm_o[16][kKvDim + 4];
   __shared__ float sm_m[16], sm_l[16];
-  int64_t u = blockIdx.x;
-  const int r16 = (int)(u % (16 * NQ));
-  u /= 16 * NQ;
-  const int64_t unit = u;
-  const int qb = (int)(u % a.nqb);
-  u /= a.nqb;
-  const int h = (int)(u % c.heads), b = (int)(u / c.heads);
+  const int per = 16 / ways, slot = grp / ways, way = grp % ways;
+  const int blocks = (a.block_rows + per - 1) / per;
+  const int64_t cut = blockIdx.x / blocks;  // the unit, counted from the first that is cut
+  const int r = (int)(blockIdx.x % blocks) * per + slot;
+  int b, h, qb;
+  kv_unit(a, a.first_split + cut, b, h, qb);
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
-  const int pr = qb * 16 * NQ + r16;
-  if (pr >= s.rows * a.group) return;
+  const int pr = qb * a.block_rows + r;
+  const bool live = r < a.block_rows && pr < s.rows * a.group;
   float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int t = grp; t < a.splits; t += 16) {
-    const int64_t at = (unit * a.splits + t) * (16 * NQ) + r16;
+  for (int t = way; live && t < a.splits; t += ways) {
+    const int64_t at = (cut * a.splits + t) * a.block_rows + r;
     const float mt = a.part_ml[2 * at], lt = a.part_ml[2 * at + 1];
     const f32x4 lo = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0);
     const f32x4 hi = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0 + 4);
@@ -459,34 +358,39 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
       acc[4 + e] = acc[4 + e] * fo + hi[e] * fn;
     }
   }
-  *reinterpret_cast<f32x4*>(&sm_o[grp][d0]) = f32x4{acc[0], acc[1], acc[2], acc[3]};
-  *reinterpret_cast<f32x4*>(&sm_o[grp][d0 + 4]) = f32x4{acc[4], acc[5], acc[6], acc[7]};
-  if (d0 == 0) {
-    sm_m[grp] = m;
-    sm_l[grp] = l;
+  if (ways > 1) {
+    *reinterpret_cast<f32x4*>(&sm_o[grp][d0]) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+    *reinterpret_cast<f32x4*>(&sm_o[grp][d0 + 4]) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+    if (d0 == 0) {
+      sm_m[grp] = m;
+      sm_l[grp] = l;
+    }
+    __syncthreads();
+    if (way != 0) return;
+    for (int g = grp + 1; g < grp + ways; ++g) m = fmaxf(m, sm_m[g]);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int g = grp; g < grp + ways; ++g) {
+      const float f = join_factor(sm_m[g], m);
+      l = __builtin_fmaf(sm_l[g], f, l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(sm_o[g][d0 + e], f, acc[e]);
+    }
   }
-  __syncthreads();
-  if (tid >= 64) return;
-  const int groups = min(a.splits, 16);
-  m = -INFINITY;
-  for (int g = 0; g < groups; ++g) m = fmaxf(m, sm_m[g]);
-  float o0 = 0.f, o1 = 0.f;
-  l = 0.f;
-  for (int g = 0; g < groups; ++g) {
-    const float f = join_factor(sm_m[g], m);
-    l = __builtin_fmaf(sm_l[g], f, l);
-    o0 = __builtin_fmaf(sm_o[g][2 * tid], f, o0);
-    o1 = __builtin_fmaf(sm_o[g][2 * tid + 1], f, o1);
-  }
+  if (!live) return;
   const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   const int row = pr / a.group, hh = h * a.group + pr % a.group;
-  *reinterpret_cast<uint32_t*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + 2 * tid) =
-      pack_bf16x2(o0 * inv, o1 * inv);
+  *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
 }
 
 struct Plan {
-  int nq, nqb, splits;
-  int64_t units, ws_bytes;
+  int nq;  // 16-row columns of the streaming form; 0: the tile form
+  int block_rows, nqb, splits;
+  int64_t units, first_split, ws_bytes;
 };
 
 int check(const dsx_kv_cache* c, const dsx_kv_batch* n, const dsx_kv_attn_params* p) {
@@ -503,36 +407,47 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   Plan r{};
   const int64_t rows = n.max_rows < p.total_rows ? n.max_rows : p.total_rows;
   const int64_t packed = rows * (p.heads_q / c.heads);
-  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : 4;
-  r.nqb = (int)((packed + 16 * r.nq - 1) / (16 * r.nq));
-  r.units = (int64_t)n.batch * c.heads * r.nqb;
   const int64_t span = p.window > 0 && p.window + rows < n.max_kv_len ? p.window + rows : n.max_kv_len;
-  const int64_t most = (span + 255) / 256;
-  const int64_t want = r.units > 0 ? (1024 + r.units - 1) / r.units : 1;
-  r.splits = (int)(want < most ? want : most);
-  if (r.splits < 1) r.splits = 1;
-  r.ws_bytes = r.splits > 1 ? r.units * r.splits * 16 * r.nq * (kKvDim + 2) * 4 : 0;
+  int cus = device_cus();
+  if (cus <= 0) cus = 256;
+  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : packed <= 64 ? 4 : 0;
+  r.block_rows = r.nq ? 16 * r.nq : kTileRows;
+  r.nqb = (int)((packed + r.block_rows - 1) / r.block_rows);
+  r.units = (int64_t)n.batch * c.heads * r.nqb;
+  r.splits = 1;
+  r.first_split = r.units;
+  if (r.nq) {
+    const int64_t most = (span + 255) / 256;
+    const int64_t want = r.units > 0 ? (4 * cus + r.units - 1) / r.units : 1;
+    r.splits = (int)(want < most ? want : most);
+    if (r.splits < 1) r.splits = 1;
+    if (r.splits > 1) r.first_split = 0;
+  } else {
+    int64_t tail;
+    kv_tile_split(r.units, span, cus, tail, r.splits);
+    r.first_split = r.units - tail;
+  }
+  r.ws_bytes = (r.units - r.first_split) * r.splits * r.block_rows * (kKvDim + 2) * 4;
   return r;
 }
 
 template <int NQ>
-void launch(const AttnArgs& a, int64_t units, hipStream_t st) {
+void launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
   kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(256), 0, st>>>(a);
-  if (a.splits > 1) kv_join_kernel<NQ><<<dim3((unsigned)(units * 16 * NQ)), dim3(256), 0, st>>>(a);
 }
 
 }  // namespace
 }  // namespace dsx
 
 extern "C" int64_t dsx_kv_attn_workspace_bytes(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
-                                                const dsx_kv_attn_params* p) {
+                                               const dsx_kv_attn_params* p) {
   using namespace dsx;
   if (check(cache, batch, p) != DSX_OK) return 0;
   return make_plan(*cache, *batch, *p).ws_bytes;
 }
 
-extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
-                                                const dsx_kv_attn_params* p, void* stream) {
+extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const dsx_kv_attn_params* p,
+                           void* stream) {
   using namespace dsx;
   const int rc = check(cache, batch, p);
   if (rc != DSX_OK) return rc;
@@ -544,31 +459,47 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
     return DSX_EALIGN;
   if (n.max_rows == 0 || p->total_rows == 0) return DSX_OK;
   Plan plan = make_plan(c, n, *p);
-  if (plan.splits > 1) {
-    if (!p->workspace)
+  if (plan.ws_bytes > 0) {
+    if (!p->workspace) {
       plan.splits = 1;
-    else if (p->workspace_bytes < plan.ws_bytes)
+      plan.first_split = plan.units;
+    } else if (p->workspace_bytes < plan.ws_bytes) {
       return DSX_EWORKSPACE;
+    }
   }
-  if (plan.units * plan.splits >= (1ll << 31) || plan.units * plan.nq * 16 >= (1ll << 31)) return DSX_EBADSHAPE;
+  const int64_t cut = plan.units - plan.first_split;
+  if (plan.units >= (1ll << 30) || cut * plan.splits * plan.block_rows >= (1ll << 31)) return DSX_EBADSHAPE;
   AttnArgs a{};
   a.c = c;
   a.n = n;
   a.p = *p;
   a.group = p->heads_q / c.heads;
   a.page_shift = __builtin_ctz((unsigned)c.page_size);
+  a.block_rows = plan.block_rows;
   a.nqb = plan.nqb;
   a.splits = plan.splits;
-  if (plan.splits > 1) {
+  a.first_split = plan.first_split;
+  if (cut > 0) {
     a.part_o = (float*)p->workspace;
-    a.part_ml = a.part_o + plan.units * plan.splits * 16 * plan.nq * kKvDim;
+    a.part_ml = a.part_o + cut * plan.splits * plan.block_rows * kKvDim;
   }
   hipStream_t st = (hipStream_t)stream;
-  if (plan.nq == 1)
-    launch<1>(a, plan.units, st);
-  else if (plan.nq == 2)
-    launch<2>(a, plan.units, st);
-  else
-    launch<4>(a, plan.units, st);
+  if (plan.nq == 1) {
+    launch_stream<1>(a, plan.units, st);
+  } else if (plan.nq == 2) {
+    launch_stream<2>(a, plan.units, st);
+  } else if (plan.nq == 4) {
+    launch_stream<4>(a, plan.units, st);
+  } else {
+    const int trc = launch_kv_tile(a, plan.units, st);
+    if (trc != DSX_OK) return trc;
+  }
+  if (hipGetLastError() != hipSuccess) return DSX_ELAUNCH;
+  if (cut > 0) {
+    int ways = 1;
+    while (ways < plan.splits && ways < 16) ways *= 2;
+    const int per = 16 / ways;
+    kv_join_kernel<<<dim3((unsigned)(cut * ((plan.block_rows + per - 1) / per))), dim3(256), 0, st>>>(a, ways);
+  }
   return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;
 }
