@@ -23,13 +23,14 @@ struct AttnArgs {
   float* part_ml;  // ((units - first_split) * splits, block_rows, 2)
 };
 
-// Unit number -> (sequence, cache head, query block).  Causal blocks come last first: they are the longest.
+// Unit number -> (sequence, cache head, query block).  Sequences inside heads: runs of units (the tile form gives each XCD
+// one) then hold all sequences alike, long and short.  Causal blocks come last first: they are the longest.
 __device__ __forceinline__ void kv_unit(const AttnArgs& a, int64_t unit, int& b, int& h, int& qb) {
   qb = (int)(unit % a.nqb);
   if (a.p.causal) qb = a.nqb - 1 - qb;
   unit /= a.nqb;
-  h = (int)(unit % a.c.heads);
-  b = (int)(unit / a.c.heads);
+  b = (int)(unit % a.n.batch);
+  h = (int)(unit / a.n.batch);
 }
 
 __device__ __forceinline__ float quad_max(float v) {  // over the four lanes n, n + 16, n + 32, n + 48
