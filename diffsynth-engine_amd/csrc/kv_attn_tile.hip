@@ -11,8 +11,10 @@
 //  * Interval kb, behind one barrier: S(kb+1)^T = K Q^T (16 MFMAs) with the rest of the exponentials of tile kb and the
 //    conversion of V(kb+1) between them, then O^T += V(kb)^T P(kb)^T (32 MFMAs) with the maximum of S(kb+1) and its first
 //    exponentials.  Two waves share a SIMD; without the interleaving both would do matrix and vector work in step.
-//  * The running maximum is a reference that moves only when a score passes it by 7 (in log2): weights are
-//    exp2(s c + e_v + 8 - m) <= 2^15, and a tile that does not move it costs no rescaling of O.
+//  * The running maximum is a reference that moves only when it has to: weights are exp2(s c + e_v + 8 - m), and only when
+//    some of them would leave fp16 (2^15) does m become the maximum so far.  A tile that does not move it costs no
+//    rescaling of O, and where a tile has one scale (pages of 64 and more) no look at its scores' maximum either: the row
+//    sums, which are needed anyway, tell.
 // LDS: K and V rows are 128 bytes; 16-byte piece j of K row r lies at j ^ (r & 7) (the permutation is applied to the
 // source address, the destination of a direct load being linear).
 #include "kv_attn_internal.h"
@@ -28,11 +30,36 @@ constexpr int kOffV = kStages * kRaw, kOffVf = 2 * kStages * kRaw, kOffFlag = kO
 constexpr int kLdsBytes = kOffFlag + 2 * 8 * 4;
 constexpr float kTileHeadroom = 8.f;       // log2 of a weight at the reference
 constexpr float kMoveAt = 7.f;             // the reference moves when a score is further above it: 8 + 7 < 16 (fp16)
+constexpr float kMostSum = 32768.f;        // a lane's weights of one tile
 constexpr float kNoRef = -3.0e38f;         // reference of a row that has seen no token: finite, so that -inf stays -inf
 
 typedef __attribute__((address_space(3))) void* lptr_t;
 
+// The kernel's own argument block, read again where it is needed: what only the rare paths use would otherwise sit in
+// scalar registers across the whole loop, and be spilled there.
+__device__ __forceinline__ const AttnArgs& args_again() {
+  auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttnArgs*)p;
+}
+// Largest of three (fmaxf twice would canonicalise its operands first).  Reads matrix results: behind mfma_settle.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm volatile("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+// The wait states between a matrix instruction and inline assembly that reads its result, which the compiler does not
+// see: 11 for the eight passes of the 16x16x128 shape.
+__device__ __forceinline__ void mfma_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 11" ::: "memory");
+}
+
+// UNI: pages of 64 tokens or more, so that a tile lies in one block and has one scale of K and one of V; otherwise every
+// 16-key group has its own.
+template <bool UNI>
 __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t units, int whole8, int cut8) {
+  constexpr int kGroups = UNI ? 1 : 4;  // scales of a tile
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const dsx_kv_cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
@@ -54,7 +81,12 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
   }
   int b, h, qb;
   kv_unit(a, unit, b, h, qb);
-  const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
+  b = __builtin_amdgcn_readfirstlane(b);
+  h = __builtin_amdgcn_readfirstlane(h);
+  qb = __builtin_amdgcn_readfirstlane(qb);
+  KvSeq s = kv_seq(a.n, b, a.p.total_rows);
+  s.rows = __builtin_amdgcn_readfirstlane(s.rows);
+  s.kv = __builtin_amdgcn_readfirstlane(s.kv);
   const int packed = s.rows * a.group;
   const int pr0 = qb * kTileRows;
   if (pr0 >= packed) return;
@@ -95,35 +127,37 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     const uint8_t* kbase = (const uint8_t*)c.k + (int64_t)h * c.k_sh;
     const uint8_t* vbase = (const uint8_t*)c.v + (int64_t)h * c.v_sh;
     const int page_mask = c.page_size - 1;
-    const int32_t* table = a.n.page_table + b * a.n.table_sb;
 
-    // Page numbers of the wave's eight keys of a tile, and the scales of a tile's four 16-key groups: 64 tiles ahead at
-    // once, one tile per lane.
+    // Page numbers of the wave's eight keys of a tile, and the scales of a tile's 16-key groups: 64 tiles ahead at once,
+    // one tile per lane.  Tiles and keys beyond the end take the last key's page: their codes are loaded and not used.
     int pg = 0, pg_at = -64;
-    auto page_of = [&](int kb) -> int {
+    auto page_of = [&](int kb) __attribute__((always_inline)) -> int {
       const int i = kb - kb_begin;
-      if (i - pg_at >= 64) {
+      if (__builtin_expect(i - pg_at >= 64, 0)) {
+        const AttnArgs& r = args_again();
         pg_at = i & ~63;
-        // (tiles and keys beyond the end take the last key's page: their codes are loaded and not used)
-        const int id = table[min((kb_begin + pg_at + lane) * KB + 8 * wave, hi_last - 1) >> a.page_shift];
-        pg = id < 0 || id >= c.pages ? 0 : id;
+        const int id = r.n.page_table[b * r.n.table_sb +
+                                      (min((kb_begin + pg_at + lane) * KB + 8 * wave, hi_last - 1) >> r.page_shift)];
+        pg = id < 0 || id >= r.c.pages ? 0 : id;
       }
       return __builtin_amdgcn_readlane(pg, i & 63);
     };
     uint32_t ks_all = 0, vs_all = 0;
     int sc_at = -64;
-    auto scales_of = [&](int kb, uint32_t& ks, uint32_t& vs) {
+    auto scales_of = [&](int kb, uint32_t& ks, uint32_t& vs) __attribute__((always_inline)) {
       const int i = kb - kb_begin;
-      if (i - sc_at >= 64) {
+      if (__builtin_expect(i - sc_at >= 64, 0)) {
+        const AttnArgs& r = args_again();
         sc_at = i & ~63;
         ks_all = vs_all = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int id = table[min((kb_begin + sc_at + lane) * KB + 16 * q, hi_last - 1) >> a.page_shift];
-          const bool bad = id < 0 || id >= c.pages;
+        for (int q = 0; q < kGroups; ++q) {
+          const int id = r.n.page_table[b * r.n.table_sb +
+                                        (min((kb_begin + sc_at + lane) * KB + 16 * q, hi_last - 1) >> r.page_shift)];
+          const bool bad = id < 0 || id >= r.c.pages;
           const int64_t page = bad ? 0 : id;
-          uint32_t k8 = ((const uint8_t*)c.k_scale)[page * c.ks_sp + h];
-          const uint32_t v8 = ((const uint8_t*)c.v_scale)[page * c.vs_sp + h];
+          uint32_t k8 = ((const uint8_t*)r.c.k_scale)[page * r.c.ks_sp + h];
+          const uint32_t v8 = ((const uint8_t*)r.c.v_scale)[page * r.c.vs_sp + h];
           if (bad || v8 == 255) k8 = 255;  // NaN scores for every row that sees the block
           ks_all |= k8 << (8 * q);
           vs_all |= v8 << (8 * q);
@@ -220,34 +254,56 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       return *reinterpret_cast<const f16x8*>(smem + kOffVf + buf * kVf + f * 1024 + lane * 16);
     };
 #define DSX_QK(S, Q, T, PART, ACC)                                                                          \
-  S[Q][T] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[T].PART, ACC, 0, 0, Q, (int)ks, 0, qf[T].s_##PART)
+  S[Q][T] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[T].PART, ACC, 0, 0, UNI ? 0 : Q, (int)ks, 0, qf[T].s_##PART)
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
 
-    auto mask = [&](f32x4 (&st)[4][2], int kb) {
+    // Position of the tile's key 4g in the row's span.  (Opaque: the differences of all 64 keys would be taken out of the
+    // loop, into registers that it needs.)
+    auto span_at = [&](int kb, int t) __attribute__((always_inline)) {
+      int at = kb * KB + 4 * g4 - my_lo[t];
+      asm volatile("" : "+v"(at));
+      return at;
+    };
+    auto mask = [&](f32x4 (&st)[4][2], int kb) __attribute__((always_inline)) {
       if (__builtin_expect(kb * KB < wlo_last || (kb + 1) * KB > whi_first, 0)) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int t = 0; t < 2; ++t) {
+          const int at = span_at(kb, t);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int key = kb * KB + 16 * q + 4 * g4 + e;
-              if ((uint32_t)(key - my_lo[t]) >= my_n[t]) st[q][t][e] = -INFINITY;
-              __builtin_amdgcn_sched_barrier(0);  // (one condition at a time: sixty-four of them take registers off the loop)
+              float x = st[q][t][e];
+              x = (uint32_t)(at + 16 * q + e) >= my_n[t] ? -INFINITY : x;
+              asm volatile("" : "+v"(x));  // (one condition at a time: all of them at once are kept in scalar registers)
+              st[q][t][e] = x;
             }
+        }
       }
     };
     // Largest s c + e_v of the lane's own keys for its two rows: a quarter of each row.
-    auto scan = [&](const f32x4 (&st)[4][2], const float (&ev)[4], float (&mx)[2]) {
+    auto scan = [&](const f32x4 (&st)[4][2], const float (&ev)[kGroups], float (&mx)[2]) __attribute__((always_inline)) {
+      mfma_settle();
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        float x[4];
+        if constexpr (UNI) {
+          float x = max3(st[0][t][0], st[0][t][1], st[0][t][2]), y = max3(st[1][t][0], st[1][t][1], st[1][t][2]);
+          x = max3(x, st[0][t][3], st[2][t][0]);
+          y = max3(y, st[1][t][3], st[3][t][0]);
+          x = max3(x, st[2][t][1], st[2][t][2]);
+          y = max3(y, st[3][t][1], st[3][t][2]);
+          x = max3(x, st[2][t][3], st[3][t][3]);
+          mx[t] = __builtin_fmaf(max3(x, y, y), cs, ev[0]);
+        } else {
+          float x[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4& v = st[q][t];
-          x[q] = __builtin_fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), cs, ev[q]);
+          for (int q = 0; q < 4; ++q) {
+            const float y = max3(st[q][t][0], st[q][t][1], st[q][t][2]);
+            x[q] = __builtin_fmaf(max3(y, y, st[q][t][3]), cs, ev[q]);
+          }
+          const float y = max3(x[0], x[1], x[2]);
+          mx[t] = max3(y, y, x[3]);
         }
-        mx[t] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
       }
     };
     auto must_move = [&](const float (&mx)[2]) {
@@ -276,9 +332,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
         }
       }
     };
-    auto scale_floats = [&](uint32_t vs, float (&ev)[4], float (&inv)[4]) {
+    auto scale_floats = [&](uint32_t vs, float (&ev)[kGroups], float (&inv)[kGroups]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < kGroups; ++q) {
         const uint32_t x = (vs >> (8 * q)) & 0xffu;
         ev[q] = (float)((int)x - 127);
         inv[q] = __uint_as_float((254u - x) << 23);
@@ -288,11 +344,11 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     // (n / 8) % 2, word (n / 2) % 4, half n % 2.  The empty asm pins each result where it is computed, between the MFMAs
     // it is written beside; the optimiser would sink it to its first use.
     float p_even = 0.f;
-    auto exp_entry = [&](const f32x4 (&st)[4][2], const float (&off)[4][2], const float (&inv)[4],
-                         uint32_t (&pw)[2][2][4], int n) {
+    auto exp_entry = [&](const f32x4 (&st)[4][2], const float (&off)[kGroups][2], const float (&inv)[kGroups],
+                         uint32_t (&pw)[2][2][4], int n) __attribute__((always_inline)) {
       const int ch = n >> 4, t = (n >> 3) & 1, w = (n >> 1) & 3, q = 2 * ch + (w >> 1);
-      float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q][t][2 * (w & 1) + (n & 1)], cs, off[q][t]));
-      lsum[t] = __builtin_fmaf(pv, inv[q], lsum[t]);
+      float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q][t][2 * (w & 1) + (n & 1)], cs, off[UNI ? 0 : q][t]));
+      lsum[t] = UNI ? lsum[t] + pv : __builtin_fmaf(pv, inv[q], lsum[t]);
       if (n & 1) {
         uint32_t word = pack_f16x2(p_even, pv);
         asm volatile("" : "+v"(word), "+v"(lsum[t]));
@@ -302,9 +358,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
         p_even = pv;
       }
     };
-    auto offsets = [&](const float (&ev)[4], float (&off)[4][2]) {
+    auto offsets = [&](const float (&ev)[kGroups], float (&off)[kGroups][2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < kGroups; ++q)
 #pragma unroll
         for (int t = 0; t < 2; ++t) off[q][t] = ev[q] + kTileHeadroom - m_ref[t];
     };
@@ -318,28 +374,30 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       for (int ch = 0; ch < 2; ++ch) {
         f16x8 seen[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+          const int at = span_at(kb, t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = kb * KB + 32 * ch + 16 * (e >> 2) + 4 * g4 + (e & 3);
-            seen[t][e] = (uint32_t)(key - my_lo[t]) < my_n[t] ? (_Float16)1.f : (_Float16)0.f;
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int e = 0; e < 8; ++e)
+            seen[t][e] = (uint32_t)(at + 32 * ch + 16 * (e >> 2) + (e & 3)) < my_n[t] ? (_Float16)1.f : (_Float16)0.f;
+        }
+        int codes = kOffV + stage * kRaw + (32 * ch + 4 * g4) * kKvDim + 8 * n16;
+        asm volatile("" : "+v"(codes));
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           f16x8 bad;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint8_t code = smem[kOffV + stage * kRaw + (32 * ch + 16 * (e >> 2) + 4 * g4 + (e & 3)) * kKvDim + 8 * n16 + i];
-            bad[e] = (code & 0x7f) == 0x7f ? (_Float16)1.f : (_Float16)0.f;
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int e = 0; e < 8; ++e)
+            bad[e] = (smem[codes + (16 * (e >> 2) + (e & 3)) * kKvDim + i] & 0x7f) == 0x7f ? (_Float16)1.f : (_Float16)0.f;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, seen[t], zero4, 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (hit[e] > 0.f) o[i][t][e] = NAN;
+            for (int e = 0; e < 4; ++e) {
+              float x = o[i][t][e];
+              x = hit[e] > 0.f ? NAN : x;
+              asm volatile("" : "+v"(x));
+              o[i][t][e] = x;
+            }
           }
         }
       }
@@ -353,11 +411,11 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
 
     f32x4 sA[4][2], sB[4][2];
     uint32_t pwA[2][2][4], pwB[2][2][4];
-    float offA[4][2], offB[4][2], invA[4], invB[4];
+    float offA[kGroups][2], offB[kGroups][2], invA[kGroups], invB[kGroups];
 
     auto interval = [&](int kb, int buf, f32x4 (&s_cur)[4][2], f32x4 (&s_next)[4][2], uint32_t (&pw_cur)[2][2][4],
-                        uint32_t (&pw_next)[2][2][4], const float (&off_cur)[4][2], const float (&inv_cur)[4],
-                        float (&off_next)[4][2], float (&inv_next)[4]) __attribute__((always_inline)) {
+                        uint32_t (&pw_next)[2][2][4], float (&off_cur)[kGroups][2],
+                        const float (&inv_cur)[kGroups], float (&off_next)[kGroups][2], float (&inv_next)[kGroups]) __attribute__((always_inline)) {
       const int i = kb - kb_begin;
       const int st1 = (i + 1) & 3, st3 = (i + 3) & 3;
       const bool more = kb + 1 < kb_end;
@@ -403,6 +461,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
               if (q == 2) DSX_QK(s_next, 2, 1, hi, s_next[2][1]);
               if (q == 3) DSX_QK(s_next, 3, 1, hi, s_next[3][1]);
             }
+            // (pinned: nothing in front of the next branch needs the products, and they would be sunk behind it, away from the
+            // vector work that is to run beside them)
+            if (x >= 2) asm volatile("" : "+v"(s_next[q][x - 2]));
             // 32 - kExpEarly entries over 16 slots
             if (n < 32) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
             if (x == 3 && n < 32) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
@@ -413,13 +474,28 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
           }
           if (q < 3) kf = kn;
         }
+        if constexpr (UNI) {
+          // A lane's sum over its keys bounds each of its weights: as long as it fits fp16, so do they, and the scores' own
+          // maximum is not needed.  Otherwise (rows that see their first token among them, their weights being inf) the
+          // scores are still there: move the references and make the tile's weights again.
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(lsum[0] > kMostSum || lsum[1] > kMostSum) != 0, 0)) {
+            const float ev[kGroups] = {(float)(127 - (int)(__float_as_uint(inv_cur[0]) >> 23))};
+            float mx[2];
+            scan(s_cur, ev, mx);
+            move(mx, pw_cur, false);
+            offsets(ev, off_cur);
+            lsum[0] = lsum[1] = 0.f;
+#pragma unroll
+            for (int n3 = 0; n3 < 32; ++n3) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n3);
+          }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          l_run[t] += lsum[t];
+          l_run[t] = UNI ? __builtin_fmaf(lsum[t], inv_cur[0], l_run[t]) : l_run[t] + lsum[t];
           lsum[t] = 0.f;
         }
         // ---- stage 2
-        float ev[4];
+        float ev[kGroups];
         scale_floats(vs, ev, inv_next);
         auto pv = [&](int f, int t) {
           if (t == 0 && f + kAhead < 16) vf[(f + kAhead) % (kAhead + 1)] = v_frag(buf, f + kAhead);
@@ -437,9 +513,11 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
           }
         if (__builtin_expect(more, 1)) {
           mask(s_next, kb + 1);
-          float mx[2];
-          scan(s_next, ev, mx);
-          if (__builtin_expect(must_move(mx), 0)) move(mx, pw_cur, true);
+          if constexpr (!UNI) {
+            float mx[2];
+            scan(s_next, ev, mx);
+            if (__builtin_expect(must_move(mx), 0)) move(mx, pw_cur, true);
+          }
         }
         offsets(ev, off_next);
         __builtin_amdgcn_sched_barrier(0);
@@ -484,7 +562,7 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
   DSX_QK(sA, Q, 1, hi, sA[Q][1]);
         DSX_FIRST(0) DSX_FIRST(1) DSX_FIRST(2) DSX_FIRST(3)
 #undef DSX_FIRST
-        float ev[4], mx[2];
+        float ev[kGroups], mx[2];
         scale_floats(vs, ev, invA);
         mask(sA, kb_begin);
         scan(sA, ev, mx);
@@ -570,14 +648,18 @@ void kv_tile_split(int64_t units, int64_t span, int cus, int64_t& tail, int& pie
 int launch_kv_tile(const AttnArgs& a, int64_t units, hipStream_t st) {
   static PerDeviceOnce attr_once;
   const int attr_rc = per_device_once(attr_once, [](int) {
-    return (int)(hipFuncSetAttribute((const void*)kv_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes) ==
-                         hipSuccess
-                     ? DSX_OK
-                     : DSX_ELAUNCH);
+    for (const void* f : {(const void*)kv_tile_kernel<true>, (const void*)kv_tile_kernel<false>})
+      if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes) != hipSuccess)
+        return (int)DSX_ELAUNCH;
+    return (int)DSX_OK;
   });
   if (attr_rc != DSX_OK) return attr_rc;
   const int64_t whole8 = (a.first_split + 7) & ~7ll, cut8 = ((units - a.first_split) * a.splits + 7) & ~7ll;
-  kv_tile_kernel<<<dim3((unsigned)(whole8 + cut8)), dim3(512), kLdsBytes, st>>>(a, units, (int)whole8, (int)cut8);
+  const dim3 grid((unsigned)(whole8 + cut8)), block(512);
+  if (a.c.page_size >= KB)
+    kv_tile_kernel<true><<<grid, block, kLdsBytes, st>>>(a, units, (int)whole8, (int)cut8);
+  else
+    kv_tile_kernel<false><<<grid, block, kLdsBytes, st>>>(a, units, (int)whole8, (int)cut8);
   return DSX_OK;
 }
 
