@@ -267,15 +267,19 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
     }
   };
 
-  TileRegs ra, rb;
-  uint32_t sa = 0, sb = 0;
-  if (tiles > 0) sa = load_tile(0, ra);
-  for (int i = 0; i < tiles; i += 2) {
-    if (i + 1 < tiles) sb = load_tile(i + 1, rb);
-    compute(i, ra, sa);
-    if (i + 1 < tiles) {
-      if (i + 2 < tiles) sa = load_tile(i + 2, ra);
-      compute(i + 1, rb, sb);
+  // kRing tiles in flight: the registers that two waves a SIMD leave unused
+  constexpr int kRing = NQ == 1 ? 3 : 2;
+  TileRegs ring[kRing];
+  uint32_t sc[kRing];
+#pragma unroll
+  for (int r = 0; r < kRing - 1; ++r)
+    if (r < tiles) sc[r] = load_tile(r, ring[r]);
+  for (int i = 0; i < tiles; i += kRing) {
+#pragma unroll
+    for (int r = 0; r < kRing; ++r) {
+      constexpr int kLast = kRing - 1;
+      if (i + r + kLast < tiles) sc[(r + kLast) % kRing] = load_tile(i + r + kLast, ring[(r + kLast) % kRing]);
+      if (i + r < tiles) compute(i + r, ring[r], sc[r]);
     }
   }
 

@@ -404,7 +404,8 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     };
 
     constexpr int kExpEarly = 12;  // entries of P(kb + 1) made in stage 2 of interval kb; even
-    constexpr int kScanFrags = 4;  // V fragments in front of the look at S(kb + 1)'s maximum
+    constexpr int kScanFrags = 4;  // V fragments in front of the look at S(kb + 1)
+    static_assert(32 - kExpEarly <= 32 && kExpEarly <= 2 * (16 - kScanFrags), "every entry has a slot");
     constexpr int kAhead = 2;      // V fragments read ahead of their MFMAs
 
 #define DSX_HEAD(N) asm volatile("s_waitcnt vmcnt(" #N ") lgkmcnt(0)\n\ts_barrier" ::: "memory")
@@ -464,9 +465,10 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
             // (pinned: nothing in front of the next branch needs the products, and they would be sunk behind it, away from the
             // vector work that is to run beside them)
             if (x >= 2) asm volatile("" : "+v"(s_next[q][x - 2]));
-            // 32 - kExpEarly entries over 16 slots
-            if (n < 32) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
-            if (x == 3 && n < 32) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
+            // 32 - kExpEarly entries spread over 16 slots
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if ((n - kExpEarly) * 16 < (4 * q + x + 1) * (32 - kExpEarly)) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
             if (q == 1 && x == 0) issue_k(st3);
             if (q == 1 && x == 2) cv_write(buf ^ 1, raw);
             if (q == 2 && x == 2) issue_v(st3);
@@ -528,7 +530,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             pv(f, t);
-            if (t == 0 && n2 < kExpEarly) exp_entry(s_next, off_next, inv_next, pw_next, n2++);
+            // kExpEarly entries spread over the slots that are left
+            if (n2 * 2 * (16 - kScanFrags) < (2 * (f - kScanFrags) + t + 1) * kExpEarly)
+              exp_entry(s_next, off_next, inv_next, pw_next, n2++);
             __builtin_amdgcn_sched_barrier(0);
           }
         if (__builtin_expect(boundary(kb), 0)) nan_rows(kb, buf, i & 3);
