@@ -2,8 +2,8 @@
 //
 // Work: a unit is (sequence, cache head, block of query rows), where the query rows of a cache head are its
 // heads_q / heads query heads times the sequence's rows, packed as row * group + head.  A workgroup walks a piece of the
-// unit's key range in tiles of 32 keys, one wave per tile, each wave with its own running maximum, sum and output; the
-// four waves meet in LDS at the end, the pieces of a split key range in a second kernel.
+// unit's key range in tiles of 32 keys, one wave per tile, each of its eight waves with a running maximum, sum and
+// output of its own; they meet in LDS at the end, the pieces of a split key range in a second kernel.
 //
 // S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4: K's codes are the operand as they lie in the cache, the page's
 // e8m0 scale rides in the instruction's scale operand, and q is the sum of two e4m3 terms with scales of their own (hi:
@@ -20,6 +20,9 @@
 // halves of a tile are the B operand of the second product as they stand.
 // A masked tile may hold NaN codes of tokens that some rows do not see: 0 * NaN must not reach those rows, so such a
 // tile takes V with the NaN replaced by 0 and adds NaN to the rows that do see it (a second product over indicators).
+#include <algorithm>
+#include <type_traits>
+
 #include "kv_attn_internal.h"
 
 namespace dsx {
@@ -35,8 +38,10 @@ struct TileRegs {
   u32x2 v[2][4];
 };
 
+constexpr int kWaves = 8;
+
 template <int NQ>  // 16-row columns of query rows
-__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -44,8 +49,17 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
   const int64_t unit = blockIdx.x / a.splits;
   int b, h, qb;
   kv_unit(a, unit, b, h, qb);
-  __shared__ float sm_o[4][16][kKvDim + 4];
-  __shared__ float sm_m[4][16], sm_l[4][16];
+  // Halves of the waves' results, lane after lane, then (row, element) by wave: never both at once.
+  __shared__ union {
+    struct {
+      f32x4 o[kWaves / 2][8][64];
+      float m[kWaves / 2][64], l[kWaves / 2][64];
+    } half;
+    struct {
+      float o[kWaves / 2][16][kKvDim + 4];
+      float m[kWaves / 2][16], l[kWaves / 2][16];
+    } row;
+  } sm;
 
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
   const int packed = s.rows * a.group;
@@ -53,66 +67,56 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
   if (pr0 >= packed) return;
 
   // ---- the rows of this block and the keys any of them sees
-  const int row_lo = pr0 / a.group, row_hi = min(pr0 + 16 * NQ, packed) - 1;
+  const int row_lo = pr0 / a.group, row_hi = (min(pr0 + 16 * NQ, packed) - 1) / a.group;
   int lo_first, hi_first, lo_last, hi_last;
   kv_row_span(s.kv, s.rows, row_lo, a.p.causal, a.p.window, lo_first, hi_first);
-  kv_row_span(s.kv, s.rows, row_hi / a.group, a.p.causal, a.p.window, lo_last, hi_last);
+  kv_row_span(s.kv, s.rows, row_hi, a.p.causal, a.p.window, lo_last, hi_last);
   const int tile_first = lo_first / kTileKeys;
   const int tile_end = (hi_last + kTileKeys - 1) / kTileKeys;
   const int per = (max(tile_end - tile_first, 0) + a.splits - 1) / a.splits;
   const int t_begin = tile_first + split * per;
   const int t_end = min(t_begin + per, tile_end);
+  // This wave's tiles t_begin + wave + kWaves i, i in [0, tiles); all rows see all keys of those in [in_lo, in_hi).
+  auto tiles_below = [&](int t) { return t > t_begin + wave ? (t - t_begin - wave + kWaves - 1) / kWaves : 0; };
+  const int tiles = tiles_below(t_end);
+  const int in_lo = min(tiles_below((lo_last + kTileKeys - 1) / kTileKeys), tiles);
+  const int in_hi = max(min(tiles_below(hi_first / kTileKeys), tiles), in_lo);
 
-  // ---- q, split into its two terms
-  QFrag qf[NQ];
+  QRaw raw[NQ];
   int my_lo[NQ], my_hi[NQ];
 #pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    load_q(a, s, h, min(pr0 + q * 16 + n16, packed - 1), g4, qf[q], my_lo[q], my_hi[q]);
-  }
-
-  f32x4 o[NQ][8];  // o[q][i][r]: query n of column q, element 32g + 8r + i
-  float m_run[NQ], l_run[NQ];
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    m_run[q] = -INFINITY;
-    l_run[q] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const float cs = a.p.softmax_scale * kLog2e;
+  for (int q = 0; q < NQ; ++q)
+    load_q(a, s, h, min(pr0 + q * 16 + n16, packed - 1), g4, raw[q], my_lo[q], my_hi[q]);
 
   const uint8_t* kbase = (const uint8_t*)c.k + (int64_t)h * c.k_sh;
   const uint8_t* vbase = (const uint8_t*)c.v + (int64_t)h * c.v_sh;
   const int koff = n16 * kKvDim + 16 * g4, voff = 4 * g4 * kKvDim + 8 * n16;
   const int page_mask = c.page_size - 1;
 
-  // Page numbers and scales of the wave's next 64 tiles, one tile per lane: two dependent loads per 64 tiles instead
-  // of two per tile.  scales: k of the halves in bytes 0, 1, v in bytes 2, 3.
-  int pg[2];
+  // Page numbers and scales of 64 of the wave's tiles, one tile per lane: two dependent loads per 64 tiles instead of two
+  // per tile.  scales: k of the halves in bytes 0, 1, v in bytes 2, 3.  Keys behind the last one take its page: what is
+  // loaded for them is not used.
+  int pg[2] = {0, 0}, pg_at = -1;
   uint32_t sc_all = 0;
-  const int tiles = t_end > t_begin + wave ? (t_end - t_begin - wave + 3) / 4 : 0;  // this wave's
-  auto preload = [&](int i0) {
-    const int t = t_begin + wave + 4 * (i0 + lane);
-    sc_all = 0x7f7f7f7fu;
+  auto preload = [&](int chunk) __attribute__((always_inline)) {
+    const AttnArgs& r = args_again();
+    pg_at = chunk;
+    sc_all = 0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int key = t * kTileKeys + 16 * hf;
-      pg[hf] = 0;
-      if (t < t_end && key < hi_last) {
-        const int id = a.n.page_table[b * a.n.table_sb + (key >> a.page_shift)];
-        const bool bad = id < 0 || id >= c.pages;
-        pg[hf] = bad ? 0 : id;
-        uint32_t ks = ((const uint8_t*)c.k_scale)[pg[hf] * c.ks_sp + h];
-        const uint32_t vs = ((const uint8_t*)c.v_scale)[pg[hf] * c.vs_sp + h];
-        if (bad || vs == 255) ks = 255;  // NaN scores for every row that sees the block
-        sc_all = (sc_all & ~(0xff00ffu << (8 * hf))) | (ks << (8 * hf)) | (vs << (16 + 8 * hf));
-      }
+      const int key = min((t_begin + wave + kWaves * (64 * chunk + lane)) * kTileKeys + 16 * hf, hi_last - 1);
+      const int id = r.n.page_table[b * r.n.table_sb + (key >> r.page_shift)];
+      const bool bad = id < 0 || id >= r.c.pages;
+      pg[hf] = bad ? 0 : id;
+      uint32_t ks = ((const uint8_t*)r.c.k_scale)[pg[hf] * r.c.ks_sp + h];
+      const uint32_t vs = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
+      if (bad || vs == 255) ks = 255;  // NaN scores for every row that sees the block
+      sc_all |= (ks << (8 * hf)) | (vs << (16 + 8 * hf));
     }
   };
-  auto load_tile = [&](int i, TileRegs& r) -> uint32_t {  // the wave's i-th tile; returns its scales
-    if ((i & 63) == 0) preload(i);
-    const int key = (t_begin + wave + 4 * i) * kTileKeys;
+  auto load_tile = [&](int i, TileRegs& r) __attribute__((always_inline)) -> uint32_t {  // returns its scales
+    if ((i >> 6) != pg_at) preload(i >> 6);
+    const int key = (t_begin + wave + kWaves * i) * kTileKeys;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int64_t page = __builtin_amdgcn_readlane(pg[hf], i & 63);
@@ -127,25 +131,50 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
     return (uint32_t)__builtin_amdgcn_readlane((int)sc_all, i & 63);
   };
 
-  auto compute = [&](int i, TileRegs& r, uint32_t sc) {
-    const int key0 = (t_begin + wave + 4 * i) * kTileKeys;
+  // ---- tiles in flight: kRing - 1 of the inner ones, and in front of them the first that has to be masked (the last of a
+  //      sequence, for most calls): it is worked on first, while the others arrive
+  constexpr int kRing = NQ == 1 ? 3 : 2;
+  TileRegs ring[kRing];
+  uint32_t sc[kRing];
+  const int first_masked = in_lo > 0 ? 0 : in_hi;
+  if (first_masked < tiles) sc[kRing - 1] = load_tile(first_masked, ring[kRing - 1]);
+#pragma unroll
+  for (int r = 0; r < kRing - 1; ++r)
+    if (in_lo + r < in_hi) sc[r] = load_tile(in_lo + r, ring[r]);
+  __builtin_amdgcn_sched_barrier(0);
+
+  QFrag qf[NQ];
+  f32x4 o[NQ][8];  // o[q][i][r]: query n of column q, element 32g + 8r + i
+  float m_run[NQ], l_run[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    split_q(raw[q], qf[q]);
+    m_run[q] = -INFINITY;
+    l_run[q] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float cs = a.p.softmax_scale * kLog2e;
+
+  auto compute = [&](auto masked, int i, TileRegs& r, uint32_t sc) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
+    const int key0 = (t_begin + wave + kWaves * i) * kTileKeys;
     f32x4 st[2][NQ];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const i32x8 kf = {(int)r.k[hf][0][0], (int)r.k[hf][0][1], (int)r.k[hf][0][2], (int)r.k[hf][0][3],
                         (int)r.k[hf][1][0], (int)r.k[hf][1][1], (int)r.k[hf][1][2], (int)r.k[hf][1][3]};
-      const int ks = (int)((sc >> (8 * hf)) & 0xffu);
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].lo, z, 0, 0, 0, ks, 0, qf[q].s_lo);
-        st[hf][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].hi, z, 0, 0, 0, ks, 0, qf[q].s_hi);
-      }
+      for (int q = 0; q < NQ; ++q)
+        st[hf][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].lo, z, 0, 0, 0, (int)(sc >> (8 * hf)), 0, qf[q].s_lo);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+        st[hf][q] =
+            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].hi, st[hf][q], 0, 0, 0, (int)(sc >> (8 * hf)), 0, qf[q].s_hi);
     }
-    // boundary tile: some row of the block does not see some key of it
-    const bool masked = key0 < lo_last || key0 + kTileKeys > hi_first;
     bool has_nan = false;
-    if (masked) {
+    if constexpr (kMasked) {
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
@@ -204,39 +233,41 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
       }
       pf[q] = __builtin_bit_cast(f16x8, pw);
     }
-    if (__builtin_expect(has_nan, 0)) {
-      f16x8 seen[NQ];
+    if constexpr (kMasked) {
+      if (__builtin_expect(has_nan, 0)) {
+        f16x8 seen[NQ];
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = key0 + 16 * (e >> 2) + 4 * g4 + (e & 3);
-          seen[q][e] = key >= my_lo[q] && key < my_hi[q] ? (_Float16)1.f : (_Float16)0.f;
-        }
-#pragma unroll
-      for (int i2 = 0; i2 < 8; ++i2) {
-        f16x8 flag;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          flag[e] = (nan_bytes(r.v[e >> 2][e & 3][i2 >> 2]) >> (8 * (i2 & 3))) & 0x80u ? (_Float16)1.f : (_Float16)0.f;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(flag, seen[q], z, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hit[e] > 0.f) o[q][i2][e] = NAN;
-        }
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t bad = nan_bytes(r.v[hf][t][w]);
-            r.v[hf][t][w] &= ~((bad >> 7) * 0xffu);
+          for (int e = 0; e < 8; ++e) {
+            const int key = key0 + 16 * (e >> 2) + 4 * g4 + (e & 3);
+            seen[q][e] = key >= my_lo[q] && key < my_hi[q] ? (_Float16)1.f : (_Float16)0.f;
           }
+#pragma unroll
+        for (int i2 = 0; i2 < 8; ++i2) {
+          f16x8 flag;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            flag[e] = (nan_bytes(r.v[e >> 2][e & 3][i2 >> 2]) >> (8 * (i2 & 3))) & 0x80u ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(flag, seen[q], z, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hit[e] > 0.f) o[q][i2][e] = NAN;
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t bad = nan_bytes(r.v[hf][t][w]);
+              r.v[hf][t][w] &= ~((bad >> 7) * 0xffu);
+            }
+      }
     }
     // V^T: row n of M-tile 4w + e is element 8n + 4w + e.  Byte pairs of two tokens come together with one permute, and
     // the converter takes either half of it.
@@ -267,65 +298,87 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void kv_stream_kernel(AttnArg
     }
   };
 
-  // kRing tiles in flight: the registers that two waves a SIMD leave unused
-  constexpr int kRing = NQ == 1 ? 3 : 2;
-  TileRegs ring[kRing];
-  uint32_t sc[kRing];
-#pragma unroll
-  for (int r = 0; r < kRing - 1; ++r)
-    if (r < tiles) sc[r] = load_tile(r, ring[r]);
-  for (int i = 0; i < tiles; i += kRing) {
+  for (int i = first_masked; i < tiles;) {
+    compute(std::true_type{}, i, ring[kRing - 1], sc[kRing - 1]);
+    ++i;
+    if (i == in_lo) i = in_hi;
+    if (i < tiles) sc[kRing - 1] = load_tile(i, ring[kRing - 1]);
+  }
+  for (int i = in_lo; i < in_hi; i += kRing) {
 #pragma unroll
     for (int r = 0; r < kRing; ++r) {
       constexpr int kLast = kRing - 1;
-      if (i + r + kLast < tiles) sc[(r + kLast) % kRing] = load_tile(i + r + kLast, ring[(r + kLast) % kRing]);
-      if (i + r < tiles) compute(i + r, ring[r], sc[r]);
+      if (i + r + kLast < in_hi) sc[(r + kLast) % kRing] = load_tile(i + r + kLast, ring[(r + kLast) % kRing]);
+      if (i + r < in_hi) compute(std::false_type{}, i + r, ring[r], sc[r]);
     }
   }
 
-  // ---- the four waves' results join in LDS, one 16-row column at a time: thread (row, 8 elements)
-  const int row16 = tid >> 4, d0 = (tid & 15) * 8;
+  // ---- the waves' results join in LDS, one 16-row column at a time: the upper half of the waves hands its lanes to the
+  //      lower half's, the rest is joined by (row, 4 elements) per thread
+  const int row16 = tid >> 5, d0 = (tid & 31) * 4;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     if (q) __syncthreads();
-    const float l = quad_sum(l_run[q]);
-    if (g4 == 0) {
-      sm_m[wave][n16] = m_run[q];
-      sm_l[wave][n16] = l;
+    if (wave >= kWaves / 2) {
+      const int w = wave - kWaves / 2;
+      sm.half.m[w][lane] = m_run[q];
+      sm.half.l[w][lane] = l_run[q];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm.half.o[w][i][lane] = o[q][i];
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 8; i += 4)
-        *reinterpret_cast<f32x4*>(&sm_o[wave][n16][32 * g4 + 8 * r + i]) =
-            f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
     __syncthreads();
-    float m = fmaxf(fmaxf(sm_m[0][row16], sm_m[1][row16]), fmaxf(sm_m[2][row16], sm_m[3][row16]));
-    float lt = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (wave < kWaves / 2) {
+      const float mb = sm.half.m[wave][lane], m = fmaxf(m_run[q], mb);
+      const float fa = join_factor(m_run[q], m), fb = join_factor(mb, m);
+      m_run[q] = m;
+      l_run[q] = l_run[q] * fa + sm.half.l[wave][lane] * fb;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = join_factor(sm_m[w][row16], m);
-      lt = __builtin_fmaf(sm_l[w][row16], f, lt);
+      for (int i = 0; i < 8; ++i) {
+        const f32x4 x = sm.half.o[wave][i][lane];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(sm_o[w][row16][d0 + e], f, acc[e]);
+        for (int e = 0; e < 4; ++e) o[q][i][e] = o[q][i][e] * fa + x[e] * fb;
+      }
+    }
+    __syncthreads();
+    if (wave < kWaves / 2) {
+      const float l = quad_sum(l_run[q]);
+      if (g4 == 0) {
+        sm.row.m[wave][n16] = m_run[q];
+        sm.row.l[wave][n16] = l;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          *reinterpret_cast<f32x4*>(&sm.row.o[wave][n16][32 * g4 + 8 * r + i]) =
+              f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
+    }
+    __syncthreads();
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves / 2; ++w) m = fmaxf(m, sm.row.m[w][row16]);
+#pragma unroll
+    for (int w = 0; w < kWaves / 2; ++w) {
+      const float f = join_factor(sm.row.m[w][row16], m);
+      l = __builtin_fmaf(sm.row.l[w][row16], f, l);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.row.o[w][row16][d0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
     }
     const int pr = pr0 + q * 16 + row16;
     if (a.splits > 1) {
       const int64_t at = (unit * a.splits + split) * (16 * NQ) + q * 16 + row16;
-#pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<f32x4*>(a.part_o + at * kKvDim + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+      *reinterpret_cast<f32x4*>(a.part_o + at * kKvDim + d0) = acc;
       if (d0 == 0) {
         a.part_ml[2 * at] = m;
-        a.part_ml[2 * at + 1] = lt;
+        a.part_ml[2 * at + 1] = l;
       }
     } else if (pr < packed) {
-      const float inv = s.ok ? (lt == 0.f ? 0.f : 1.f / lt) : NAN;
-      u32x4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
+      const u32x2 w = {pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
       const int row = pr / a.group, hh = h * a.group + pr % a.group;
-      *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+      *reinterpret_cast<u32x2*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
     }
   }
 }
@@ -414,17 +467,18 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   const int64_t span = p.window > 0 && p.window + rows < n.max_kv_len ? p.window + rows : n.max_kv_len;
   int cus = device_cus();
   if (cus <= 0) cus = 256;
-  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : packed <= 64 ? 4 : 0;
+  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : 0;
   r.block_rows = r.nq ? 16 * r.nq : kTileRows;
   r.nqb = (int)((packed + r.block_rows - 1) / r.block_rows);
   r.units = (int64_t)n.batch * c.heads * r.nqb;
   r.splits = 1;
   r.first_split = r.units;
   if (r.nq) {
-    const int64_t most = (span + 255) / 256;
-    const int64_t want = r.units > 0 ? (4 * cus + r.units - 1) / r.units : 1;
-    r.splits = (int)(want < most ? want : most);
-    if (r.splits < 1) r.splits = 1;
+    const int64_t tiles = (span + kTileKeys - 1) / kTileKeys;
+    int64_t s = 1;
+    if (r.units > 0 && r.units < cus) s = std::min<int64_t>(cus / r.units, tiles / 16);
+    else if (r.units > 0 && r.units < 4 * cus) s = std::min<int64_t>((4 * cus + r.units - 1) / r.units, tiles / 1000000);
+    r.splits = s < 1 ? 1 : (int)s;
     if (r.splits > 1) r.first_split = 0;
   } else {
     int64_t tail;
@@ -437,7 +491,7 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
 
 template <int NQ>
 void launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
-  kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(256), 0, st>>>(a);
+  kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
 }
 
 }  // namespace
@@ -492,8 +546,6 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
     launch_stream<1>(a, plan.units, st);
   } else if (plan.nq == 2) {
     launch_stream<2>(a, plan.units, st);
-  } else if (plan.nq == 4) {
-    launch_stream<4>(a, plan.units, st);
   } else {
     const int trc = launch_kv_tile(a, plan.units, st);
     if (trc != DSX_OK) return trc;

@@ -93,24 +93,35 @@ __device__ __forceinline__ void split_q(const float (&x)[32], QFrag& f) {
 }
 
 // Packed query row `pr` of a cache head: its span and its operand (the lane's elements 16g .. +15 and 64 + 16g .. +15).
-__device__ __forceinline__ void load_q(const AttnArgs& a, const KvSeq& s, int h, int pr, int g4, QFrag& f, int& lo,
+struct QRaw {
+  u32x4 w[4];
+};
+__device__ __forceinline__ void load_q(const AttnArgs& a, const KvSeq& s, int h, int pr, int g4, QRaw& raw, int& lo,
                                        int& hi) {
   const int row = pr / a.group, hh = h * a.group + pr % a.group;
   kv_row_span(s.kv, s.rows, row, a.p.causal, a.p.window, lo, hi);
   const uint16_t* src = (const uint16_t*)a.p.q + (int64_t)(s.row0 + row) * a.p.q_sr + hh * a.p.q_sh + 16 * g4;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) raw.w[w] = *reinterpret_cast<const u32x4*>(src + 64 * (w >> 1) + 8 * (w & 1));
+}
+__device__ __forceinline__ void split_q(const QRaw& raw, QFrag& f) {
   float x[32];
 #pragma unroll
-  for (int half = 0; half < 2; ++half)
+  for (int w = 0; w < 4; ++w)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 64 * half + 8 * w);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[16 * half + 8 * w + 2 * j] = bf16_lo(raw[j]);
-        x[16 * half + 8 * w + 2 * j + 1] = bf16_hi(raw[j]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      x[8 * w + 2 * j] = bf16_lo(raw.w[w][j]);
+      x[8 * w + 2 * j + 1] = bf16_hi(raw.w[w][j]);
     }
   split_q(x, f);
+}
+
+// A kernel's own argument block, read again where it is needed: what only the rare paths use would otherwise sit in
+// scalar registers across the whole loop, and be spilled there.  (AttnArgs is the first argument of both kernels.)
+__device__ __forceinline__ const AttnArgs& args_again() {
+  auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttnArgs*)p;
 }
 
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // 0x80 in every byte that holds e4m3's NaN

@@ -35,13 +35,6 @@ constexpr float kNoRef = -3.0e38f;         // reference of a row that has seen n
 
 typedef __attribute__((address_space(3))) void* lptr_t;
 
-// The kernel's own argument block, read again where it is needed: what only the rare paths use would otherwise sit in
-// scalar registers across the whole loop, and be spilled there.
-__device__ __forceinline__ const AttnArgs& args_again() {
-  auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const AttnArgs*)p;
-}
 // Largest of three (fmaxf twice would canonicalise its operands first).  Reads matrix results: behind mfma_settle.
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
@@ -111,7 +104,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     int end;
-    load_q(a, s, h, min(wr0 + 16 * t + n16, packed - 1), g4, qf[t], my_lo[t], end);
+    QRaw raw;
+    load_q(a, s, h, min(wr0 + 16 * t + n16, packed - 1), g4, raw, my_lo[t], end);
+    split_q(raw, qf[t]);
     my_n[t] = (uint32_t)(end - my_lo[t]);
   }
 
