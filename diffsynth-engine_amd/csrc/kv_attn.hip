@@ -40,15 +40,46 @@ struct TileRegs {
 
 constexpr int kWaves = 8;
 
+// ---- Equal shares.  The tiles of all units lie behind one another, head by head and sequence by sequence, and are dealt
+// to `share` workgroups in equal runs whatever the sequences' lengths (which only the device knows): a run may end inside
+// a unit, and then both sides leave partial results.  Every wave sums the lengths for itself, a sequence per lane.
+__device__ __forceinline__ int span_tiles(const AttnArgs& a, const KvSeq& s) {  // tiles that any row of a sequence sees
+  int lo, hi, unused;
+  kv_row_span(s.kv, s.rows, 0, a.p.causal, a.p.window, lo, unused);
+  kv_row_span(s.kv, s.rows, s.rows - 1, a.p.causal, a.p.window, unused, hi);
+  return s.rows == 0 ? 0 : max((hi + kTileKeys - 1) / kTileKeys - lo / kTileKeys, 0);
+}
+struct Lens {     // 64 sequences from b0 on, one per lane
+  int b0, count, upto;  // the lane's tiles; the sum over the lanes up to it
+  KvSeq s;
+};
+__device__ __forceinline__ void load_lens(const AttnArgs& a, int b0, int lane, Lens& x) {
+  x.b0 = b0;
+  x.s = kv_seq(a.n, min(b0 + lane, a.n.batch - 1), a.p.total_rows);
+  x.count = b0 + lane < a.n.batch ? span_tiles(a, x.s) : 0;
+  x.upto = wave_scan(x.count);
+}
+__device__ __forceinline__ int head_sum(const AttnArgs& a, int lane, Lens& x) {  // tiles of one head; leaves x at b0 = 0
+  int sum = 0;
+  for (int b0 = (a.n.batch - 1) & ~63; b0 >= 0; b0 -= 64) {
+    load_lens(a, b0, lane, x);
+    sum += __builtin_amdgcn_readlane(x.upto, 63);
+  }
+  return sum;
+}
+// Runs of `total` tiles: workgroup w of n takes [share_begin(w), share_begin(w + 1)).  No run is shorter than two tiles a
+// wave: below that, what a piece costs besides its tiles is most of its time.
+__device__ __forceinline__ int share_count(int total, int n) { return min(n, max(total / (2 * kWaves), 1)); }
+__device__ __forceinline__ int share_begin(int total, int n, int w) { return w * (total / n) + w * (total % n) / n; }
+__device__ __forceinline__ int share_of(int total, int n, int x) {  // whose run holds tile x
+  return (int)((((uint64_t)x + 1) * n - 1) / (uint64_t)total);
+}
+
 template <int NQ>  // 16-row columns of query rows
 __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = (int)(blockIdx.x % a.splits);
-  const int64_t unit = blockIdx.x / a.splits;
-  int b, h, qb;
-  kv_unit(a, unit, b, h, qb);
   // Halves of the waves' results, lane after lane, then (row, element) by wave: never both at once.
   __shared__ union {
     struct {
@@ -61,21 +92,72 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     } row;
   } sm;
 
-  const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
+  // This workgroup's tiles among all of them, as head and place in the head (one whole unit: nothing to look up).
+  int h = 0, place = 0, left = 1, head_tiles = 1;
+  Lens lens;
+  if (a.share) {
+    head_tiles = head_sum(a, lane, lens);
+    const int total = head_tiles * c.heads;
+    if (total == 0) return;
+    const int n = share_count(total, a.share);
+    if ((int)blockIdx.x >= n) return;
+    place = share_begin(total, n, blockIdx.x);
+    left = share_begin(total, n, blockIdx.x + 1) - place;
+    h = place / head_tiles;
+    place -= h * head_tiles;
+  }
+  for (bool again = false; left > 0; again = true) {
+  // ---- the next segment: a whole unit or a part of one
+  int b, qb = 0, skip = 0, count = 0x3fffffff, piece = -1;  // piece: where a part's result goes
+  KvSeq s;
+  if (a.share) {
+    if (place == head_tiles) {
+      place = 0;
+      ++h;
+    }
+    int before = 0;  // tiles of the sequences in front of the 64 at hand
+    uint64_t beyond;
+    if (lens.b0 != 0) load_lens(a, 0, lane, lens);
+    while ((beyond = __builtin_amdgcn_ballot_w64(before + lens.upto > place)) == 0) {
+      before += __builtin_amdgcn_readlane(lens.upto, 63);
+      load_lens(a, lens.b0 + 64, lane, lens);
+    }
+    const int at = __builtin_ctzll(beyond);
+    b = lens.b0 + at;
+    s.row0 = __builtin_amdgcn_readlane(lens.s.row0, at);
+    s.rows = __builtin_amdgcn_readlane(lens.s.rows, at);
+    s.kv = __builtin_amdgcn_readlane(lens.s.kv, at);
+    s.ok = true;  // (one that is not has no tiles)
+    const int all = __builtin_amdgcn_readlane(lens.count, at);
+    skip = place - (before + __builtin_amdgcn_readlane(lens.upto, at) - all);
+    count = min(all - skip, left);
+    if (count < all) piece = 2 * blockIdx.x + (skip == 0);
+    place += count;
+    left -= count;
+  } else {
+    kv_unit(a, blockIdx.x / a.splits, b, h, qb);
+    s = kv_seq(a.n, b, a.p.total_rows);
+    left = 0;
+  }
   const int packed = s.rows * a.group;
   const int pr0 = qb * 16 * NQ;
   if (pr0 >= packed) return;
+  if (again) __syncthreads();  // the LDS of the segment before
 
   // ---- the rows of this block and the keys any of them sees
   const int row_lo = pr0 / a.group, row_hi = (min(pr0 + 16 * NQ, packed) - 1) / a.group;
   int lo_first, hi_first, lo_last, hi_last;
   kv_row_span(s.kv, s.rows, row_lo, a.p.causal, a.p.window, lo_first, hi_first);
   kv_row_span(s.kv, s.rows, row_hi, a.p.causal, a.p.window, lo_last, hi_last);
-  const int tile_first = lo_first / kTileKeys;
   const int tile_end = (hi_last + kTileKeys - 1) / kTileKeys;
-  const int per = (max(tile_end - tile_first, 0) + a.splits - 1) / a.splits;
-  const int t_begin = tile_first + split * per;
-  const int t_end = min(t_begin + per, tile_end);
+  int t_begin = lo_first / kTileKeys;
+  if (a.splits > 1) {
+    count = (max(tile_end - t_begin, 0) + a.splits - 1) / a.splits;
+    skip = (int)(blockIdx.x % a.splits) * count;
+    piece = blockIdx.x;
+  }
+  t_begin += skip;
+  const int t_end = min(t_begin + count, tile_end);
   // This wave's tiles t_begin + wave + kWaves i, i in [0, tiles); all rows see all keys of those in [in_lo, in_hi).
   auto tiles_below = [&](int t) { return t > t_begin + wave ? (t - t_begin - wave + kWaves - 1) / kWaves : 0; };
   const int tiles = tiles_below(t_end);
@@ -315,7 +397,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 
   // ---- the waves' results join in LDS, one 16-row column at a time: the upper half of the waves hands its lanes to the
   //      lower half's, the rest is joined by (row, 4 elements) per thread
-  const int row16 = tid >> 5, d0 = (tid & 31) * 4;
+  const int d0 = (tid & 31) * 4;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     if (q) __syncthreads();
@@ -354,32 +436,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
               f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
     }
     __syncthreads();
-    float m = -INFINITY, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int row16 = tid >> 5; row16 < 16; row16 += 2 * kWaves) {
+      float m = -INFINITY, l = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves / 2; ++w) m = fmaxf(m, sm.row.m[w][row16]);
+      for (int w = 0; w < kWaves / 2; ++w) m = fmaxf(m, sm.row.m[w][row16]);
 #pragma unroll
-    for (int w = 0; w < kWaves / 2; ++w) {
-      const float f = join_factor(sm.row.m[w][row16], m);
-      l = __builtin_fmaf(sm.row.l[w][row16], f, l);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.row.o[w][row16][d0]);
+      for (int w = 0; w < kWaves / 2; ++w) {
+        const float f = join_factor(sm.row.m[w][row16], m);
+        l = __builtin_fmaf(sm.row.l[w][row16], f, l);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.row.o[w][row16][d0]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
-    }
-    const int pr = pr0 + q * 16 + row16;
-    if (a.splits > 1) {
-      const int64_t at = (unit * a.splits + split) * (16 * NQ) + q * 16 + row16;
-      *reinterpret_cast<f32x4*>(a.part_o + at * kKvDim + d0) = acc;
-      if (d0 == 0) {
-        a.part_ml[2 * at] = m;
-        a.part_ml[2 * at + 1] = l;
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
       }
-    } else if (pr < packed) {
-      const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
-      const u32x2 w = {pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
-      const int row = pr / a.group, hh = h * a.group + pr % a.group;
-      *reinterpret_cast<u32x2*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+      const int pr = pr0 + q * 16 + row16;
+      if (piece >= 0) {
+        const int64_t at = (int64_t)piece * (16 * NQ) + q * 16 + row16;
+        *reinterpret_cast<f32x4*>(a.part_o + at * kKvDim + d0) = acc;
+        if (d0 == 0) {
+          a.part_ml[2 * at] = m;
+          a.part_ml[2 * at + 1] = l;
+        }
+      } else if (pr < packed) {
+        const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
+        const u32x2 w = {pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+        const int row = pr / a.group, hh = h * a.group + pr % a.group;
+        *reinterpret_cast<u32x2*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+      }
     }
+  }
   }
 }
 
@@ -399,9 +484,34 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
   const int pr = qb * a.block_rows + r;
   const bool live = r < a.block_rows && pr < s.rows * a.group;
+  // Pieces of the unit: number t at piece0 + t * step, the first one place later.
+  int pieces = a.splits, step = 1, odd = 0;
+  int64_t piece0 = cut * a.splits;
+  if (a.share) {
+    const int lane = tid & 63;
+    Lens lens;
+    const int head_tiles = head_sum(a, lane, lens), total = head_tiles * a.c.heads;
+    int first = h * head_tiles;
+    for (int b0 = 0; b0 + 64 <= b; b0 += 64) {
+      first += __builtin_amdgcn_readlane(lens.upto, 63);
+      load_lens(a, b0 + 64, lane, lens);
+    }
+    const int count = __builtin_amdgcn_readlane(lens.count, b & 63);
+    first += __builtin_amdgcn_readlane(lens.upto, b & 63) - count;
+    pieces = 0;
+    if (count > 0) {
+      const int n = share_count(total, a.share);
+      const int w0 = share_of(total, n, first), w1 = share_of(total, n, first + count - 1);
+      if (w0 == w1) return;  // one workgroup had all of it and wrote the result
+      pieces = w1 - w0 + 1;  // the first workgroup's piece begins the unit, the others' continue it
+      piece0 = 2 * (int64_t)w0;
+      step = 2;
+      odd = 1;
+    }
+  }
   float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int t = way; live && t < a.splits; t += ways) {
-    const int64_t at = (cut * a.splits + t) * a.block_rows + r;
+  for (int t = way; live && t < pieces; t += ways) {
+    const int64_t at = (piece0 + (int64_t)t * step + (t == 0 ? odd : 0)) * a.block_rows + r;
     const float mt = a.part_ml[2 * at], lt = a.part_ml[2 * at + 1];
     const f32x4 lo = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0);
     const f32x4 hi = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0 + 4);
@@ -446,8 +556,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
 
 struct Plan {
   int nq;  // 16-row columns of the streaming form; 0: the tile form
-  int block_rows, nqb, splits;
-  int64_t units, first_split, ws_bytes;
+  int block_rows, nqb, share, splits, ways;
+  int64_t units, first_split, join_units, ws_bytes;
 };
 
 int check(const dsx_kv_cache* c, const dsx_kv_batch* n, const dsx_kv_attn_params* p) {
@@ -473,25 +583,42 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   r.units = (int64_t)n.batch * c.heads * r.nqb;
   r.splits = 1;
   r.first_split = r.units;
+  r.ways = 1;
+  int64_t pieces = 0;
   if (r.nq) {
-    const int64_t tiles = (span + kTileKeys - 1) / kTileKeys;
-    int64_t s = 1;
-    if (r.units > 0 && r.units < cus) s = std::min<int64_t>(cus / r.units, tiles / 16);
-    else if (r.units > 0 && r.units < 4 * cus) s = std::min<int64_t>((4 * cus + r.units - 1) / r.units, tiles / 1000000);
-    r.splits = s < 1 ? 1 : (int)s;
-    if (r.splits > 1) r.first_split = 0;
+    const int64_t tiles = (span + kTileKeys - 1) / kTileKeys + 1;
+    const int64_t load = r.units * tiles / cus;  // of a compute unit, at most
+    if (load >= 512 && r.units * tiles < (1ll << 30)) {
+      r.share = cus;
+      pieces = 2 * (int64_t)r.share;
+      r.ways = (int)((r.share + r.units - 1) / r.units) + 1;
+    } else if (r.units < cus && r.units > 0) {
+      r.splits = (int)std::max<int64_t>(std::min<int64_t>(cus / r.units, tiles / 8), 1);
+      if (r.splits > 1) pieces = r.units * r.splits;
+      r.ways = r.splits;
+    }
+    if (pieces > 0) {
+      r.first_split = 0;
+      r.join_units = r.units;
+    }
   } else {
     int64_t tail;
     kv_tile_split(r.units, span, cus, tail, r.splits);
     r.first_split = r.units - tail;
+    pieces = tail * r.splits;
+    r.join_units = tail;
+    r.ways = r.splits;
   }
-  r.ws_bytes = (r.units - r.first_split) * r.splits * r.block_rows * (kKvDim + 2) * 4;
+  int ways = 1;
+  while (ways < r.ways && ways < 16) ways *= 2;
+  r.ways = ways;
+  r.ws_bytes = pieces * r.block_rows * (kKvDim + 2) * 4;
   return r;
 }
 
 template <int NQ>
 void launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
-  kv_stream_kernel<NQ><<<dim3((unsigned)(units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
+  kv_stream_kernel<NQ><<<dim3((unsigned)(a.share ? a.share : units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
 }
 
 }  // namespace
@@ -520,13 +647,16 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
   if (plan.ws_bytes > 0) {
     if (!p->workspace) {
       plan.splits = 1;
+      plan.share = 0;
       plan.first_split = plan.units;
+      plan.join_units = 0;
     } else if (p->workspace_bytes < plan.ws_bytes) {
       return DSX_EWORKSPACE;
     }
   }
-  const int64_t cut = plan.units - plan.first_split;
-  if (plan.units >= (1ll << 30) || cut * plan.splits * plan.block_rows >= (1ll << 31)) return DSX_EBADSHAPE;
+  const int per = 16 / plan.ways;
+  const int64_t join_wgs = plan.join_units * ((plan.block_rows + per - 1) / per);
+  if (plan.units >= (1ll << 30) || join_wgs >= (1ll << 31)) return DSX_EBADSHAPE;
   AttnArgs a{};
   a.c = c;
   a.n = n;
@@ -535,11 +665,12 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
   a.page_shift = __builtin_ctz((unsigned)c.page_size);
   a.block_rows = plan.block_rows;
   a.nqb = plan.nqb;
+  a.share = plan.share;
   a.splits = plan.splits;
   a.first_split = plan.first_split;
-  if (cut > 0) {
+  if (plan.join_units > 0) {
     a.part_o = (float*)p->workspace;
-    a.part_ml = a.part_o + cut * plan.splits * plan.block_rows * kKvDim;
+    a.part_ml = a.part_o + plan.ws_bytes / (4 * (kKvDim + 2)) * kKvDim;
   }
   hipStream_t st = (hipStream_t)stream;
   if (plan.nq == 1) {
@@ -551,11 +682,6 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
     if (trc != DSX_OK) return trc;
   }
   if (hipGetLastError() != hipSuccess) return DSX_ELAUNCH;
-  if (cut > 0) {
-    int ways = 1;
-    while (ways < plan.splits && ways < 16) ways *= 2;
-    const int per = 16 / ways;
-    kv_join_kernel<<<dim3((unsigned)(cut * ((plan.block_rows + per - 1) / per))), dim3(256), 0, st>>>(a, ways);
-  }
+  if (join_wgs > 0) kv_join_kernel<<<dim3((unsigned)join_wgs), dim3(256), 0, st>>>(a, plan.ways);
   return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;
 }

@@ -17,10 +17,11 @@ struct AttnArgs {
   int page_shift;
   int block_rows;  // packed query rows of a unit
   int nqb;         // query blocks per (sequence, cache head)
-  int64_t first_split;  // units from this one on are cut
+  int share;       // streaming form: 0, or the number of workgroups that share all units' tiles evenly
+  int64_t first_split;  // tile form: units from this one on are cut
   int splits;           // into so many pieces of their key ranges
-  float* part_o;   // ((units - first_split) * splits, block_rows, 128) fp32
-  float* part_ml;  // ((units - first_split) * splits, block_rows, 2)
+  float* part_o;   // (pieces, block_rows, 128) fp32
+  float* part_ml;  // (pieces, block_rows, 2)
 };
 
 // Unit number -> (sequence, cache head, query block).  Sequences inside heads: runs of units (the tile form gives each XCD
@@ -31,6 +32,21 @@ __device__ __forceinline__ void kv_unit(const AttnArgs& a, int64_t unit, int& b,
   unit /= a.nqb;
   b = (int)(unit % a.n.batch);
   h = (int)(unit / a.n.batch);
+}
+
+// Inclusive sum over the lanes of a wave: six adds, each fed by the row shifts and broadcasts of the vector unit.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8: inside rows of 16
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast15 into rows 1 and 3
+  v = dpp_add<0x143, 0xc>(v);  // row_bcast31 into rows 2 and 3
+  return v;
 }
 
 __device__ __forceinline__ float quad_max(float v) {  // over the four lanes n, n + 16, n + 32, n + 48
