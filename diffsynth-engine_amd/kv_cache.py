@@ -47,7 +47,7 @@ class KVCache:
             raise ValueError("KVCache: too many pages")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page_size, _ = k.shape
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._c = _lib.KVCacheParams(
             k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(),
             k_sp=k.stride(0), k_sh=k.stride(1), v_sp=v.stride(0), v_sh=v.stride(1), ks_sp=k_scale.stride(0),
@@ -93,7 +93,7 @@ class KVPlan:
         self.page_table, self.row_start, self.kv_len = page_table, row_start, kv_len
         self.batch, self.table_pages = page_table.shape
         self.max_rows, self.max_kv_len = int(max_rows), int(max_kv_len)
-        self.device = kv_len.device
+        self.device, self._index = kv_len.device, kv_len.get_device()
         self._c = _lib.KVBatchParams(
             page_table=page_table.data_ptr(), table_sb=max(page_table.stride(0), self.table_pages),
             row_start=row_start.data_ptr(), kv_len=kv_len.data_ptr(), batch=self.batch, table_pages=self.table_pages,
@@ -118,8 +118,8 @@ class KVPlan:
             raise ValueError("KVPlan: sequence %d (rows [%d, %d), %d tokens) breaks a bound"
                              % (b, starts[b], starts[b + 1], lens[b]) if b >= 0 else _lib.strerror(rc))
 
-    def _fits(self, cache: KVCache, device: Optional[torch.device] = None):
-        if cache.device != self.device or (device is not None and device != self.device):
+    def _fits(self, cache: KVCache, index: Optional[int] = None):
+        if cache._index != self._index or (index is not None and index != self._index):
             raise ValueError("the rows, the cache and the plan must be on one device")
         if self.max_kv_len > self.table_pages * cache.page_size:
             raise ValueError("KVPlan: %d pages of %d tokens cannot hold max_kv_len = %d"

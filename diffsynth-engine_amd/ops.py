@@ -4,7 +4,6 @@ PyTorch is used for device memory and the current stream only; every function be
 hand-written gfx950 kernels from libdsx.so on ``torch.cuda.current_stream()`` and raises if the
 library is missing or the tensors are not on a GPU.
 """
-import contextlib
 import ctypes
 import math
 from typing import Optional, Tuple
@@ -644,10 +643,11 @@ def flow_match_euler_step(latents: torch.Tensor, model_outputs: torch.Tensor, dt
 
 def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None):
     """(pointer, row stride, head stride) of a (rows, heads, 128) bf16 view."""
-    if t.dtype != _BF16 or t.dim() != 3 or t.shape[0] != rows or t.shape[2] != HEAD_DIM \
-            or (heads is not None and t.shape[1] != heads):
+    shape = t.shape
+    if t.dtype != _BF16 or len(shape) != 3 or shape[0] != rows or shape[2] != HEAD_DIM \
+            or (heads is not None and shape[1] != heads):
         raise ValueError("%s must be bf16 (%d, %s, 128), got %s %s"
-                         % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(t.shape)))
+                         % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(shape)))
     sr, sh, sd = t.stride()
     ptr = t.data_ptr()
     if sd != 1 or sr % 8 or sh % 8 or ptr % 16:
@@ -656,9 +656,36 @@ def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None)
     return ptr, sr, sh
 
 
-def _on(device: torch.device):
-    """Makes the tensors' device the current one where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _kv_device(name: str, cache: KVCache, plan: KVPlan, *tensors) -> int:
+    """The one device that everything is on (a number: these calls are short, and device objects take a while)."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _require_cuda(*tensors)
+            raise ValueError("%s: all tensors must be on one device" % name)
+    if index < 0:
+        _require_cuda(*tensors)
+    plan._fits(cache, index)
+    return index
+
+
+def _kv_call(fn, what: str, index: int, *args):
+    """Calls the library with the tensors' device current and that device's current stream."""
+    if index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
+    else:
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
+
+
+def _kv_norm_weight(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if w is None:
+        return None
+    if w.numel() != HEAD_DIM:
+        raise ValueError("kv_append: RMSNorm weights have 128 entries")
+    if w.dtype != _BF16 or not w.is_contiguous():
+        w = w.to(_BF16).contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
@@ -679,43 +706,36 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
     not appended (``plan.check`` finds them); rows behind the last sequence are left alone, in q_out too.
 
     Returns q prepared (``q_out`` or a new tensor; q_out may be q), or None without q."""
-    _require_cuda(k, v, q, q_out, k_norm_w, q_norm_w, rope)
-    plan._fits(cache, k.device)
+    index = _kv_device("kv_append", cache, plan, k, v, q, q_out, k_norm_w, q_norm_w, rope)
+    if k.dim() != 3:
+        raise ValueError("kv_append: k must be (rows, heads, 128)")
     rows = k.shape[0]
-    P = _lib.KVAppendParams(total_rows=rows, norm_eps=eps)
-    P.k, P.k_sr, P.k_sh = _kv_rows("kv_append: k", k, rows, cache.heads)
-    P.v, P.v_sr, P.v_sh = _kv_rows("kv_append: v", v, rows, cache.heads)
+    kp, k_sr, k_sh = _kv_rows("kv_append: k", k, rows, cache.heads)
+    vp, v_sr, v_sh = _kv_rows("kv_append: v", v, rows, cache.heads)
     if not eps >= 0:
         raise ValueError("kv_append: eps must not be negative")
-    keep = []
+    qp = qop = None
+    q_sr = q_sh = qo_sr = qo_sh = heads = 0
     if q is None:
         if q_norm_w is not None or q_out is not None:
             raise ValueError("kv_append: q_norm_w and q_out go with q")
     else:
-        P.q, P.q_sr, P.q_sh = _kv_rows("kv_append: q", q, rows)
-        P.heads_q = q.shape[1]
+        qp, q_sr, q_sh = _kv_rows("kv_append: q", q, rows)
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
-        P.q_out, P.qo_sr, P.qo_sh = _kv_rows("kv_append: q_out", q_out, rows, q.shape[1])
-    for name, w in (("k_norm_w", k_norm_w), ("q_norm_w", q_norm_w)):
-        if w is not None:
-            if w.numel() != HEAD_DIM:
-                raise ValueError("kv_append: RMSNorm weights have 128 entries")
-            w = w.to(_BF16).contiguous()
-            if w.data_ptr() % 16:
-                w = w.clone()
-            keep.append(w)
-            setattr(P, name, w.data_ptr())
+            q_out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
+        qop, qo_sr, qo_sh = _kv_rows("kv_append: q_out", q_out, rows, heads)
+    k_norm_w, q_norm_w = _kv_norm_weight(k_norm_w), _kv_norm_weight(q_norm_w)
+    rope_sb = rope_rows = 0
     if rope is not None:
         rope = _rope_table(rope, plan.batch, plan.max_kv_len)
-        keep.append(rope)
-        P.rope, P.rope_rows = rope.data_ptr(), rope.shape[1]
-        P.rope_sb = rope.stride(0) if rope.shape[0] > 1 else 0
-    if any(t is not None and t.device != k.device for t in (v, q, q_out, k_norm_w, q_norm_w, rope)):
-        raise ValueError("kv_append: all tensors must be on one device")
-    if rows and (P.heads_q or q is None):
-        with _on(k.device):
-            _lib.check(_lib.load().dsx_kv_append(cache._ref, plan._ref, ctypes.byref(P), _stream()), "dsx_kv_append")
+        rope_rows = rope.shape[1]
+        rope_sb = rope.stride(0) if rope.shape[0] > 1 else 0
+    if not rows or (q is not None and not heads):
+        return q_out
+    p = _lib.KVAppendParams(kp, k_sr, k_sh, vp, v_sr, v_sh, qp, q_sr, q_sh, qop, qo_sr, qo_sh, _ptr(k_norm_w),
+                            _ptr(q_norm_w), _ptr(rope), rope_sb, rope_rows, rows, eps, heads)
+    _kv_call(_lib.load().dsx_kv_append, "dsx_kv_append", index, cache._ref, plan._ref, ctypes.byref(p))
     return q_out
 
 
@@ -733,31 +753,29 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     out of range.  Rows of ``out`` behind the last sequence are left as they are (and hold nothing meaningful in an
     ``out`` made here).  Where units of work are few, their key ranges are split over the chip through a workspace
     allocated here (split_keys=False: never)."""
-    _require_cuda(q, out)
-    plan._fits(cache, q.device)
-    rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    P = _lib.KVAttnParams(total_rows=rows, heads_q=heads, causal=int(bool(causal)), window=window,
-                          softmax_scale=1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
-    P.q, P.q_sr, P.q_sh = _kv_rows("kv_attention: q", q, rows)
+    index = _kv_device("kv_attention", cache, plan, q, out)
+    if q.dim() != 3:
+        raise ValueError("kv_attention: q must be (rows, heads, 128)")
+    rows, heads, _ = q.shape
+    qp, q_sr, q_sh = _kv_rows("kv_attention: q", q, rows)
     if heads < 1 or heads % cache.heads:
         raise ValueError("kv_attention: %d query heads for %d cache heads" % (heads, cache.heads))
     if window < 0 or window > 0x7fffffff:
         raise ValueError("kv_attention: window must lie in [0, 2^31)")
-    if not 0.0 < P.softmax_scale < math.inf:
+    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
         raise ValueError("kv_attention: scale must be positive and finite")
     if out is None:
         out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
-    elif out.device != q.device:
-        raise ValueError("kv_attention: all tensors must be on one device")
-    P.out, P.o_sr, P.o_sh = _kv_rows("kv_attention: out", out, rows, heads)
+    op, o_sr, o_sh = _kv_rows("kv_attention: out", out, rows, heads)
     if not rows:
         return out
     lib = _lib.load()
-    with _on(q.device):
-        p = ctypes.byref(P)
-        need = lib.dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, p) if split_keys else 0
-        if need > 0:
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-            P.workspace, P.workspace_bytes = ws.data_ptr(), need
-        _lib.check(lib.dsx_kv_attn(cache._ref, plan._ref, p, _stream()), "dsx_kv_attn")
+    p = _lib.KVAttnParams(qp, q_sr, q_sh, op, o_sr, o_sh, rows, scale, heads, bool(causal), window, None, 0)
+    ref = ctypes.byref(p)
+    need = lib.dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, ref) if split_keys else 0
+    if need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    _kv_call(lib.dsx_kv_attn, "dsx_kv_attn", index, cache._ref, plan._ref, ref)
     return out
