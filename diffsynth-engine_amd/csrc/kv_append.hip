@@ -1,14 +1,17 @@
 // Appending a batch's keys and values to the paged 8-bit cache, and its queries' normalisation and rotation.
 //
-// One workgroup = one (page, head) block of K or of V, or 64 (row, head) pairs of q.  A block's tokens are held in
+// One workgroup = one (page, head) block of K or of V, or 16 rows x kQHeads heads of q.  A block's tokens are held in
 // registers between the two passes over them (largest magnitude, then codes), so each element is read once and written
-// once: 16 lanes per token, 8 elements per lane, page/16 tokens per lane.
+// once: 16 lanes per token, 8 elements per lane, page/16 tokens per lane.  A row of q keeps its line of the rotation table in
+// registers for kQHeads heads.
 #include <stdlib.h>
 
 #include "kv_internal.h"
 
 namespace dsx {
 namespace {
+
+constexpr int kQHeads = 4;
 
 struct AppendArgs {
   dsx_kv_cache c;
@@ -37,29 +40,32 @@ __device__ __forceinline__ void load8(const uint16_t* src, float (&x)[8]) {
   }
 }
 
-// RMSNorm over the head, then the rotation of pairs (2i, 2i + 1): lane `ln` of the token's 16 holds elements 8 ln ..
-__device__ __forceinline__ void norm_rope(float (&x)[8], const uint16_t* w, float eps, const float* rope_row, int ln) {
-  if (w) {
-    float ss = 0.f;
+// RMSNorm over the head, then the rotation of pairs (2i, 2i + 1): the lane's place in the token's 16 is its elements 8 ln ..
+// and cs the (cos, sin) of its four pairs.
+__device__ __forceinline__ void load_turn(const float* rope_row, int ln, float (&cs)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln);
+  const f32x4 b = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln + 4);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-    const float r = 1.0f / sqrtf(row16_sum(ss) * (1.0f / kKvDim) + eps);
-    float g[8];
-    load8(w + 8 * ln, g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= r * g[j];
+  for (int j = 0; j < 4; ++j) {
+    cs[j] = a[j];
+    cs[4 + j] = b[j];
   }
-  if (rope_row) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln);
-    const f32x4 b = *reinterpret_cast<const f32x4*>(rope_row + 8 * ln + 4);
-    const float cs[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+__device__ __forceinline__ void turn(float (&x)[8], const float (&cs)[8]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x0 = x[2 * j], x1 = x[2 * j + 1], c = cs[2 * j], s = cs[2 * j + 1];
-      x[2 * j] = x0 * c - x1 * s;
-      x[2 * j + 1] = x0 * s + x1 * c;
-    }
+  for (int j = 0; j < 4; ++j) {
+    const float x0 = x[2 * j], x1 = x[2 * j + 1], c = cs[2 * j], s = cs[2 * j + 1];
+    x[2 * j] = x0 * c - x1 * s;
+    x[2 * j + 1] = x0 * s + x1 * c;
   }
+}
+__device__ __forceinline__ void norm(float (&x)[8], const float (&g)[8], float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+  const float r = __builtin_amdgcn_rsqf(row16_sum(ss) * (1.0f / kKvDim) + eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] *= r * g[j];
 }
 
 // value * 2^-e as the clamp's operand: saturates at +-448 (infinities too), NaN stays NaN
@@ -77,24 +83,28 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   __shared__ uint32_t smax[4];
 
   if ((int64_t)blockIdx.x >= a.q_begin) {
-    const int64_t u = (int64_t)blockIdx.x - a.q_begin;
-    const int b = (int)(u / a.q_per_seq), chunk = (int)(u % a.q_per_seq);
+    const unsigned u = blockIdx.x - (unsigned)a.q_begin;
+    const int b = (int)(u / (unsigned)a.q_per_seq), chunk = (int)(u % (unsigned)a.q_per_seq);
     const KvSeq s = kv_seq(n, b, p.total_rows);
     if (!s.ok || s.kv < s.rows) return;
-    const int64_t pairs = (int64_t)s.rows * p.heads_q;
+    const int per_row = (p.heads_q + kQHeads - 1) / kQHeads;
+    const int at = chunk * 16 + grp, row = at / per_row, h0 = at % per_row * kQHeads;
+    if (row >= s.rows) return;
+    const uint16_t* src = (const uint16_t*)p.q + (int64_t)(s.row0 + row) * p.q_sr + 8 * ln;
+    uint16_t* dst = (uint16_t*)p.q_out + (int64_t)(s.row0 + row) * p.qo_sr + 8 * ln;
+    float x[kQHeads][8], g[8], cs[8];
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int64_t pr = (int64_t)chunk * 64 + it * 16 + grp;
-      if (pr >= pairs) return;
-      const int row = (int)(pr / p.heads_q), h = (int)(pr % p.heads_q);
-      float x[8];
-      load8((const uint16_t*)p.q + (int64_t)(s.row0 + row) * p.q_sr + h * p.q_sh + 8 * ln, x);
-      const float* rr = p.rope ? p.rope + b * p.rope_sb + (int64_t)(s.kv - s.rows + row) * kKvDim : nullptr;
-      norm_rope(x, (const uint16_t*)p.q_norm_w, p.norm_eps, rr, ln);
+    for (int i = 0; i < kQHeads; ++i) load8(src + min(h0 + i, p.heads_q - 1) * p.q_sh, x[i]);
+    if (p.q_norm_w) load8((const uint16_t*)p.q_norm_w + 8 * ln, g);
+    if (p.rope) load_turn(p.rope + b * p.rope_sb + (int64_t)(s.kv - s.rows + row) * kKvDim, ln, cs);
+#pragma unroll
+    for (int i = 0; i < kQHeads; ++i) {
+      if (p.q_norm_w) norm(x[i], g, p.norm_eps);
+      if (p.rope) turn(x[i], cs);
       u32x4 w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
-      *reinterpret_cast<u32x4*>((uint16_t*)p.q_out + (int64_t)(s.row0 + row) * p.qo_sr + h * p.qo_sh + 8 * ln) = w;
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[i][2 * j], x[i][2 * j + 1]);
+      if (h0 + i < p.heads_q) *reinterpret_cast<u32x4*>(dst + (h0 + i) * p.qo_sh) = w;
     }
     return;
   }
@@ -114,15 +124,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   const int base = pi << a.page_shift;  // the block's first token
   if (base >= s.kv || s.rows == 0) return;
   const int id = n.page_table[b * n.table_sb + pi];
-  if (id < 0 || id >= c.pages) return;
   const int lo = first > base ? first - base : 0;  // tokens [lo, hi) of the block are new, [0, lo) stay
   const int hi = s.kv - base < page ? s.kv - base : page;
 
   const uint16_t* src = is_v ? (const uint16_t*)p.v + h * p.v_sh : (const uint16_t*)p.k + h * p.k_sh;
   const int64_t sr = is_v ? p.v_sr : p.k_sr;
-  uint8_t* codes = is_v ? (uint8_t*)c.v + id * c.v_sp + h * c.v_sh : (uint8_t*)c.k + id * c.k_sp + h * c.k_sh;
-  uint8_t* scale = is_v ? (uint8_t*)c.v_scale + id * c.vs_sp + h : (uint8_t*)c.k_scale + id * c.ks_sp + h;
-
   float x[TOK][8];
   float amax = 0.f;
 #pragma unroll
@@ -135,12 +141,25 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
       for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
     }
   }
-  if (!is_v && (p.k_norm_w || p.rope)) {
+  // (the rows are under way before the page number that they go to is looked at)
+  if (id < 0 || id >= c.pages) return;
+  uint8_t* codes = is_v ? (uint8_t*)c.v + id * c.v_sp + h * c.v_sh : (uint8_t*)c.k + id * c.k_sp + h * c.k_sh;
+  uint8_t* scale = is_v ? (uint8_t*)c.v_scale + id * c.vs_sp + h : (uint8_t*)c.k_scale + id * c.ks_sp + h;
+  if (!is_v && p.k_norm_w) {
+    float g[8];
+    load8((const uint16_t*)p.k_norm_w + 8 * ln, g);
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) norm(x[i], g, p.norm_eps);
+  }
+  if (!is_v && p.rope) {
 #pragma unroll
     for (int i = 0; i < TOK; ++i) {
       const int t = grp + 16 * i;
-      const float* rr = p.rope && t >= lo && t < hi ? p.rope + b * p.rope_sb + (int64_t)(base + t) * kKvDim : nullptr;
-      norm_rope(x[i], (const uint16_t*)p.k_norm_w, p.norm_eps, rr, ln);
+      if (t >= lo && t < hi) {
+        float cs[8];
+        load_turn(p.rope + b * p.rope_sb + (int64_t)(base + t) * kKvDim, ln, cs);
+        turn(x[i], cs);
+      }
     }
   }
 #pragma unroll
@@ -245,9 +264,9 @@ extern "C" int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batc
   a.blocks_per_seq = (int)((rows + c.page_size - 2) / c.page_size + 1);
   const int64_t kv_wgs = (int64_t)n.batch * a.blocks_per_seq * c.heads * 2;
   a.q_begin = kv_wgs;
-  const int64_t q_per_seq = p->q ? (rows * p->heads_q + 63) / 64 : 0;
+  const int64_t q_per_seq = p->q ? (rows * ((p->heads_q + kQHeads - 1) / kQHeads) + 15) / 16 : 0;
   const int64_t total = kv_wgs + (int64_t)n.batch * q_per_seq;
-  if (total >= (1ll << 31) || q_per_seq >= (1ll << 31)) return DSX_EBADSHAPE;
+  if (total >= (1ll << 31) || q_per_seq >= (1ll << 27)) return DSX_EBADSHAPE;
   a.q_per_seq = (int)q_per_seq;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)total), block(256);

@@ -577,7 +577,12 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   const int64_t span = p.window > 0 && p.window + rows < n.max_kv_len ? p.window + rows : n.max_kv_len;
   int cus = device_cus();
   if (cus <= 0) cus = 256;
-  r.nq = packed <= 16 ? 1 : packed <= 32 ? 2 : 0;
+  // 16 rows to a column of the matrix instruction.  From 33 to 64 rows, two blocks of two columns while those leave compute
+  // units free and the cache is short (8 x 5 rows, group 7, window 4096: 31 us against the tile form's 36); otherwise the
+  // tile form (64 x 8 rows, group 5, 2048 tokens: 90 against 135 us; 1 x 60, 40 heads, 65536 tokens: 215 against 230).
+  const int64_t blocks2 = 2ll * n.batch * c.heads;
+  const bool few = blocks2 <= cus && blocks2 * span / kTileKeys < 64ll * cus;
+  r.nq = packed <= 16 ? 1 : packed <= 32 || (packed <= 64 && few) ? 2 : 0;
   r.block_rows = r.nq ? 16 * r.nq : kTileRows;
   r.nqb = (int)((packed + r.block_rows - 1) / r.block_rows);
   r.units = (int64_t)n.batch * c.heads * r.nqb;
@@ -587,13 +592,18 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   int64_t pieces = 0;
   if (r.nq) {
     const int64_t tiles = (span + kTileKeys - 1) / kTileKeys + 1;
-    const int64_t load = r.units * tiles / cus;  // of a compute unit, at most
-    if (load >= 512 && r.units * tiles < (1ll << 30)) {
+    // The longest a compute unit's share can be, in tiles.  From 512 on, even shares and a join (which costs 6 us) beat one
+    // workgroup per unit and its uneven end: 64 x 16384 tokens, 8 heads (1024 tiles): 288 against 305 us; 32 x 16384 (512):
+    // 173 against 178; 32 x 8192 (256): 93 against 90; 32 x 4097 (129): 58 against 46.  Fewer units than compute units are
+    // cut into equal pieces of at least a tile a wave (pieces of two or four tiles bring nothing: 1561 tokens, 12 heads,
+    // 13.3 against 13.6 and 14.5 us).
+    const int64_t load = r.units * tiles / cus;
+    if (load >= 512 && r.nqb == 1 && r.units * tiles < (1ll << 30)) {
       r.share = cus;
       pieces = 2 * (int64_t)r.share;
       r.ways = (int)((r.share + r.units - 1) / r.units) + 1;
     } else if (r.units < cus && r.units > 0) {
-      r.splits = (int)std::max<int64_t>(std::min<int64_t>(cus / r.units, tiles / 8), 1);
+      r.splits = (int)std::max<int64_t>(std::min<int64_t>(cus / r.units, tiles / kWaves), 1);
       if (r.splits > 1) pieces = r.units * r.splits;
       r.ways = r.splits;
     }
