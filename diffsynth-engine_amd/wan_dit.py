@@ -15,6 +15,10 @@ along as extra latent channels, the CLIP feature goes through the ``img_emb`` ML
 front of the text context, and every cross-attention adds a second attention of the same queries over those rows
 (own k/v projections and k norm) before the o projection.
 
+Frame by frame: with a ``WanFrameCache`` a call computes a run of frames that attends to itself and to the frames in front
+of it, whose keys and values the cache holds in 8 bits per block, instead of the whole video at once.  The reference has
+no counterpart.
+
 The reference wires FP8 for Flux only (models/flux/flux_dit.py:404; pipelines/base.py:164-165 raises for the
 rest); here every Linear of the Wan DiT runs through the same scaled e4m3 GEMM as Flux.
 """
@@ -24,6 +28,7 @@ from typing import Dict, Optional
 import torch
 
 from . import ops
+from .kv_cache import KVCache, KVPlan
 from .flux_dit import _Linear, _gemm_pair, count_blocks, ingest_state_dict
 
 
@@ -48,6 +53,32 @@ def wan_config_from_shapes(shapes: Dict[str, tuple], eps: float = 1e-6) -> dict:
             "freq_dim": shapes["time_embedding.0.weight"][1], "eps": eps, "patch_size": patch,
             "num_heads": dim // 128, "num_layers": layers,
             "has_image_input": "img_emb.proj.1.weight" in shapes}
+
+
+class WanFrameCache:
+    """Self-attention keys and values of a video's frames so far, 8 bits wide, one ``KVCache`` per block of the model
+    (``WanDiTRunner.frame_cache`` makes it).  ``frames``: how many frames (in tokens' time steps) it holds."""
+
+    def __init__(self, layers: int, heads: int, frames: int, h: int, w: int, batch: int, page_size: int, device):
+        if min(layers, heads, frames, h, w, batch) < 1:
+            raise ValueError("WanFrameCache: every size must be at least 1")
+        self.max_frames, self.h, self.w, self.batch, self.frames = frames, h, w, batch, 0
+        pages = -(-frames * h * w // page_size)
+        self.layers = [KVCache.empty(batch * pages, heads, page_size, device) for _ in range(layers)]
+        self.table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
+
+    def bytes(self) -> int:
+        return sum(t.numel() for c in self.layers for t in (c.k, c.v, c.k_scale, c.v_scale))
+
+    def plan(self, first: int, frames: int) -> KVPlan:
+        """The batch of a call that computes frames [first, first + frames)."""
+        if not 0 <= first <= self.frames or frames < 1 or first + frames > self.max_frames:
+            raise ValueError("WanFrameCache: frames [%d, %d) do not continue the %d that are held (of %d at most)"
+                             % (first, first + frames, self.frames, self.max_frames))
+        rows, tokens = frames * self.h * self.w, (first + frames) * self.h * self.w
+        starts = torch.arange(0, (self.batch + 1) * rows, rows, dtype=torch.int32, device=self.table.device)
+        lens = torch.full((self.batch,), tokens, dtype=torch.int32, device=self.table.device)
+        return KVPlan(self.table, starts, lens, max_rows=rows, max_kv_len=tokens)
 
 
 class WanDiTRunner:
@@ -89,17 +120,24 @@ class WanDiTRunner:
         return ops.adaln_modulate(x, scale, shift, self.cfg["eps"], ln_weight=w, ln_bias=b, want_bf16=False,
                                   want_fp8=True, scaled=self.scaled)
 
-    def rope_table(self, f, h, w, theta=10000.0):
+    def frame_cache(self, frames: int, height: int, width: int, batch: int = 1, page_size: int = 64) -> WanFrameCache:
+        """A cache for ``forward(..., cache=, first_frame=)``: room for ``frames`` latent frames of height x width
+        (latent sizes, as in ``x``)."""
+        pf, ph, pw = self.cfg["patch_size"]
+        return WanFrameCache(self.cfg["num_layers"], self.cfg["num_heads"], frames // pf, height // ph, width // pw,
+                             batch, page_size, self.device)
+
+    def rope_table(self, f, h, w, theta=10000.0, first=0):
         """(1, f*h*w, 64, 2) fp32 (cos, sin): head dim split (d - 2*(d//3), d//3, d//3) over (frame, row, col)
-        with float64 angles pos * theta^(-2j/dim_axis) (wan_dit.py:38-51,335-346)."""
+        with float64 angles pos * theta^(-2j/dim_axis) (wan_dit.py:38-51,335-346); frames from ``first`` on."""
         hd = self.cfg["dim"] // self.cfg["num_heads"]
         dev = self.device
 
-        def axis(dim, end):
+        def axis(dim, end, start=0):
             fr = 1.0 / (theta ** (torch.arange(0, dim, 2, device=dev)[: dim // 2].double() / dim))
-            return torch.outer(torch.arange(end, device=dev).double(), fr)
+            return torch.outer(torch.arange(start, end, device=dev).double(), fr)
 
-        af, ah, aw = axis(hd - 2 * (hd // 3), f), axis(hd // 3, h), axis(hd // 3, w)
+        af, ah, aw = axis(hd - 2 * (hd // 3), first + f, first), axis(hd // 3, h), axis(hd // 3, w)
         ang = torch.cat([af.view(f, 1, 1, -1).expand(f, h, w, -1), ah.view(1, h, 1, -1).expand(f, h, w, -1),
                          aw.view(1, 1, w, -1).expand(f, h, w, -1)], dim=-1).reshape(1, f * h * w, -1)
         return torch.stack((torch.cos(ang), torch.sin(ang)), dim=-1).float().contiguous()
@@ -129,9 +167,10 @@ class WanDiTRunner:
             parts.append(None if t is None else self._q(t.reshape(B * t.shape[1], d)) + (t.shape[1],))
         return parts
 
-    def block(self, i, x, context, t_mod, rope, context_q=None):
+    def block(self, i, x, context, t_mod, rope, context_q=None, kv=None):
         """DiTBlock.forward; x (B,S,d), context (B,Sc,d) already embedded, t_mod (B,6,d); ``context_q``: what
-        quantise_context(context) returned, when the caller has it already."""
+        quantise_context(context) returned, when the caller has it already; ``kv``: (KVCache, KVPlan) that x's keys and
+        values join and its queries attend to, instead of x's own alone."""
         p = f"blocks.{i}."
         L, V, eps = self.lin, self.vec, self.cfg["eps"]
         B, S, d = x.shape
@@ -144,13 +183,19 @@ class WanDiTRunner:
         # The RMSNorm runs over all heads at once, so no static bound on a head's scores exists; the norm kernels
         # leave the largest squared head norm of q and of k on the device and the attention kernels read it there
         # (|q.k| <= |q||k|): with ordinary activations the running softmax maximum is not needed.
-        nm = torch.zeros(2, dtype=torch.float32, device=x.device) if self.device_score_bound else None
+        nm = torch.zeros(2, dtype=torch.float32, device=x.device) if self.device_score_bound and kv is None else None
         q = ops.rmsnorm_rows(L[p + "self_attn.q"](hq, hs).view(B, S, d), V[p + "self_attn.norm_q.weight"], eps, rope,
                              head_norm2_max=None if nm is None else nm[0:1])
         k = ops.rmsnorm_rows(L[p + "self_attn.k"](hq, hs).view(B, S, d), V[p + "self_attn.norm_k.weight"], eps, rope,
                              head_norm2_max=None if nm is None else nm[1:2])
         v = L[p + "self_attn.v"](hq, hs).view(B, S, d)
-        aq, asc = self._q(self._attention(q, k, v, nm))
+        if kv is None:
+            a = self._attention(q, k, v, nm)
+        else:
+            heads = lambda t: t.view(B * S, -1, 128)
+            ops.kv_append(heads(k), heads(v), *kv)
+            a = ops.kv_attention(heads(q), *kv, causal=False).view(B * S, d)
+        aq, asc = self._q(a)
         x2 = L[p + "self_attn.o"](aq, asc, resid=x2, gate=m[2], rows_per_batch=S)
         # cross-attention (no gate on the residual)
         hq, hs = self._modulate_q(x2.view(B, S, d), None, None, V[p + "norm3.weight"], V[p + "norm3.bias"])
@@ -187,8 +232,14 @@ class WanDiTRunner:
                                   ln_bias=V["img_emb.proj.4.bias"])
 
     @torch.no_grad()
-    def forward(self, x, context, timestep, clip_feature=None, y=None):
-        """``clip_feature`` (B,257,clip_dim) and ``y`` (B,c_y,f,h,w): the image-to-video inputs (both or neither)."""
+    def forward(self, x, context, timestep, clip_feature=None, y=None, cache: Optional[WanFrameCache] = None,
+                first_frame: int = 0):
+        """``clip_feature`` (B,257,clip_dim) and ``y`` (B,c_y,f,h,w): the image-to-video inputs (both or neither).
+
+        ``cache``: x holds the latent frames [first_frame, first_frame + x.shape[2]) of a longer video.  They attend to
+        one another and to the frames in front of them, as the cache has them; their own keys and values replace what it
+        holds from first_frame on.  A denoising loop calls this with the same first_frame for every step of a run of
+        frames, and goes on behind them when they are done."""
         cfg = self.cfg
         d = cfg["dim"]
         pf, ph, pw = cfg["patch_size"]
@@ -210,12 +261,24 @@ class WanDiTRunner:
             ctx = torch.cat([self._img_emb(clip_feature), ctx], dim=1)  # image rows first           (:333)
         B, C, Fr, Hh, Ww = x.shape
         f, h, w = Fr // pf, Hh // ph, Ww // pw
+        first, plan = 0, None
+        if cache is None:
+            if first_frame:
+                raise ValueError("first_frame goes with a cache")
+        else:
+            if (cache.batch, cache.h, cache.w, len(cache.layers)) != (B, h, w, cfg["num_layers"]) or first_frame % pf:
+                raise ValueError("the cache was made for a batch of %d, %d x %d tokens a frame and %d blocks"
+                                 % (cache.batch, cache.h, cache.w, len(cache.layers)))
+            first = first_frame // pf
+            plan = cache.plan(first, f)
         patches = x.to(bf).view(B, C, f, pf, h, ph, w, pw).permute(0, 2, 4, 6, 1, 3, 5, 7)
         hs = self._linear_bf16(patches.reshape(B, f * h * w, C * pf * ph * pw), "patch_embedding")
-        rope = self.rope_table(f, h, w)
+        rope = self.rope_table(f, h, w, first=first)
         ctx_q = self.quantise_context(ctx)
         for i in range(cfg["num_layers"]):
-            hs = self.block(i, hs, ctx, t_mod, rope, ctx_q)
+            hs = self.block(i, hs, ctx, t_mod, rope, ctx_q, None if cache is None else (cache.layers[i], plan))
+        if cache is not None:
+            cache.frames = first + f
         # Head.forward (wan_dit.py:234-237).  The reference adds the (B, d) embedding to the (1, 2, d) table as it
         # stands, so a batch of two (its batched classifier-free guidance, pipelines/wan_video.py:233-248, where both
         # entries carry the same timestep) gets ONE (shift, scale) pair, shift from entry 0 and scale from entry 1;
