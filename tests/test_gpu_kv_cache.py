@@ -540,3 +540,136 @@ def test_refusals(dev):
     none = q[:0]
     assert ops.kv_attention(none, c.cache, c.plan).shape == none.shape
     assert ops.kv_append(k[:0], v[:0], c.cache, c.plan) is None
+
+
+class Pool:
+    """Random pages that the page tables of many sequences share, and the same formulas in 64 bits on the device."""
+
+    def __init__(self, dev, heads, pages, page, seed=0):
+        from diffsynth_engine_amd import kv_cache
+
+        self.dev, self.page, self.heads, self.g = dev, page, heads, torch.Generator(dev).manual_seed(seed)
+        put = lambda scale: (torch.randn(pages, heads, page, 128, generator=self.g, device=dev) * scale).clamp(-448, 448).to(F8)
+        self.codes = put(128.0), put(200.0)  # times 2^-7 below: keys of deviation 1
+        v_exp = torch.randint(-12, 1, (pages, heads), generator=self.g, device=dev)
+        self.exps = torch.full_like(v_exp, -7), v_exp
+        self.cache = kv_cache.KVCache(*self.codes, *[(e + 127).to(torch.uint8).view(E8) for e in self.exps])
+
+    def batch(self, rows, lens, group):
+        """(plan, starts, table, q)"""
+        from diffsynth_engine_amd import kv_cache
+
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=self.dev)
+        starts = [0]
+        for r in rows:
+            starts.append(starts[-1] + r)
+        width = -(-max(lens) // self.page)
+        table = torch.randint(0, self.codes[0].shape[0], (len(rows), width), generator=self.g, device=self.dev).int()
+        q = torch.randn(starts[-1], self.heads * group, 128, generator=self.g, device=self.dev).bfloat16()
+        return kv_cache.KVPlan(table, ints(starts), ints(lens), max_rows=max(rows), max_kv_len=max(lens)), starts, table, q
+
+    def value(self, i, pages, n):
+        """(heads, n, 128) fp64 of the first n tokens on these pages"""
+        held = pages[: -(-n // self.page)].long()
+        x = self.codes[i][held].double() * torch.exp2(self.exps[i][held].double())[..., None, None]
+        return x.transpose(0, 1).flatten(1, 2)[:, :n].contiguous()
+
+    def check(self, out, q, starts, table, lens, causal=True, window=0, only=None):
+        group = q.shape[1] // self.heads
+        for b in range(len(lens)) if only is None else only:
+            r, n = starts[b + 1] - starts[b], lens[b]
+            if r == 0:
+                continue
+            got = out[starts[b]:starts[b + 1]].double()
+            if n == 0:
+                assert (got == 0).all()
+                continue
+            k, v = self.value(0, table[b], n), self.value(1, table[b], n)
+            end = torch.arange(n - r + 1, n + 1, device=self.dev) if causal else torch.full((r,), n, device=self.dev)
+            pos = torch.arange(n, device=self.dev)
+            see = pos < end[:, None]
+            if window:
+                see &= pos >= end[:, None] - window
+            for h in range(self.heads):
+                x = q[starts[b]:starts[b + 1], h * group:(h + 1) * group].double().transpose(0, 1).flatten(0, 1)
+                s = x @ k[h].t().contiguous() / math.sqrt(128)
+                p = torch.softmax(s.masked_fill(~see.repeat(group, 1), -math.inf), -1)
+                p = torch.where(see.repeat(group, 1), p, 0.0)  # rows that see nothing
+                want, size = (p @ v[h]).view(group, r, 128), (p @ v[h].abs()).view(group, r, 128)
+                off = (got[:, h * group:(h + 1) * group].transpose(0, 1) - want).abs()
+                assert (off - (2.0 ** -8 * want.abs() + 2.0 ** -9 * size)).max().item() <= 0, (b, h)
+
+
+@pytest.mark.parametrize("batch,heads,group,top,most_rows", [
+    (70, 8, 4, 16384, 3),     # long ragged caches
+    (700, 8, 1, 1700, 1),     # many sequences
+    (66, 32, 5, 4097, 3),     # two units meet in one share
+    (1, 40, 1, 150000, 1),    # few units: every share is a piece of one
+])
+def test_even_shares_of_long_caches(dev, batch, heads, group, top, most_rows):
+    # more than 512 tiles of 32 tokens for every compute unit, by the plan's own bounds
+    from diffsynth_engine_amd import ops
+
+    g = torch.Generator().manual_seed(batch)
+    pool = Pool(dev, heads, 64, 64, seed=batch)
+    lens = torch.randint(0, top + 1, (batch,), generator=g).tolist()
+    lens[0] = top
+    rows = [min(int(r), n) if i % 5 else 1 for i, (r, n) in enumerate(zip(torch.randint(0, most_rows + 1, (batch,), generator=g),
+                                                                          lens))]
+    plan, starts, table, q = pool.batch(rows, lens, group)
+    cus = torch.cuda.get_device_properties(dev).multi_processor_count
+    if batch > 1:
+        assert batch * heads * (top // 32 + 1) >= 512 * cus
+    for kw in (dict(), dict(window=1000), dict(causal=False)):
+        out = ops.kv_attention(q, pool.cache, plan, **kw)
+        pool.check(out, q, starts, table, lens, only=None if batch <= 70 and not kw else range(0, batch, 13), **kw)
+        assert torch.equal(out, ops.kv_attention(q, pool.cache, plan, **kw))
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("rows,lens,heads,group,kw", [
+    ([300, 257], [9001, 4200], 1, 1, {}),                       # tile form, page numbers loaded more than once
+    ([300], [9001], 1, 1, dict(causal=False, split_keys=False)),
+    ([3, 1], [40001, 16500], 2, 2, dict(split_keys=False)),     # streaming form, the same
+    ([8], [20000], 2, 4, dict(window=17000, split_keys=False)),
+    ([9, 5], [3000, 700], 4, 7, {}),                            # two blocks of two columns
+    ([60], [2000], 3, 1, {}),
+    ([33, 1], [1000, 2000], 2, 1, dict(causal=False)),
+    ([900], [1700], 5, 20, {}),                                 # units behind the last whole round are cut
+    ([900], [1700], 5, 20, dict(causal=False, window=1200)),
+])
+def test_long_key_ranges_and_forms_in_between(dev, page, rows, lens, heads, group, kw):
+    from diffsynth_engine_amd import ops
+
+    pool = Pool(dev, heads, 100, page, seed=page)
+    plan, starts, table, q = pool.batch(rows, lens, group)
+    out = ops.kv_attention(q, pool.cache, plan, **kw)
+    kw = {n: x for n, x in kw.items() if n != "split_keys"}
+    pool.check(out, q, starts, table, lens, **kw)
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("rows", [1, 20, 50, 300])
+@pytest.mark.parametrize("shape", ["rise", "fall", "spike", "late"])
+def test_scores_that_move_the_reference(dev, page, rows, shape):
+    # Scores up to |q| |k| = 128 * 6 / sqrt(128) = 68 for the row that agrees with u.  The terms of the bound above:
+    # scale |q|max sum|k| 2^-22 = 0.09 * 5 * 900 * 2^-22 < 2^-13, scale sum|q k| 2^-17 < 85 * 2^-17 < 2^-10.5 and 2^-15:
+    # 2 d + 2^-11 < 2^-9.4 + 2^-11 + 2^-11.4 < 2^-8.5; the third term of `close` is taken twice for it.
+    c = Case(dev, [rows], [max(rows, 1) + 1500], page=page, seed=rows)
+    n, g = c.lens[0], c.g
+    u = torch.randn(128, generator=g).sign()
+    t = torch.arange(n, dtype=torch.float32)
+    height = {"rise": 6 * t / n, "fall": 6 - 6 * t / n, "spike": 6.0 * (t == 700), "late": 6.0 * (t >= n - rows - 40)}[shape]
+    k = height[:, None, None] * u + 0.25 * torch.randn(n, 2, 128, generator=g)
+    for p, at in enumerate(c.table[0]):
+        x = k[p * page:(p + 1) * page] * 16  # e4m3's normal numbers: exponent -4 below
+        c.host["k"][at, :, :x.shape[0]] = x.transpose(0, 1).to(F8)
+    c.host["k_scale"].fill_(-4)
+    c.cache.k.copy_(c.host["k"].to(dev))
+    c.cache.k_scale.view(torch.uint8).fill_(123)
+    sign = torch.tensor([1.0, -1.0, 0.1])[torch.arange(c.total) % 3]
+    c.q = (sign[:, None, None] * u + 0.05 * torch.randn(c.total, 2, 128, generator=g)).bfloat16()
+    for causal in (True, False):
+        got = c.attend(causal=causal)
+        want, size = c.want(causal=causal)
+        close(got, want, 2 * size, c.starts[-1])
