@@ -6,6 +6,8 @@
 // registers for kQHeads heads.
 #include <stdlib.h>
 
+#include <algorithm>
+
 #include "kv_internal.h"
 
 namespace dsx {
@@ -259,14 +261,14 @@ extern "C" int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batc
   a.n = n;
   a.p = *p;
   a.page_shift = __builtin_ctz((unsigned)c.page_size);
-  const int64_t rows = n.max_rows < n.max_kv_len ? n.max_rows : n.max_kv_len;
+  const int64_t rows = std::min<int64_t>({n.max_rows, n.max_kv_len, p->total_rows});
   if (rows == 0) return DSX_OK;
   a.blocks_per_seq = (int)((rows + c.page_size - 2) / c.page_size + 1);
   const int64_t kv_wgs = (int64_t)n.batch * a.blocks_per_seq * c.heads * 2;
   a.q_begin = kv_wgs;
   const int64_t q_per_seq = p->q ? (rows * ((p->heads_q + kQHeads - 1) / kQHeads) + 15) / 16 : 0;
   const int64_t total = kv_wgs + (int64_t)n.batch * q_per_seq;
-  if (total >= (1ll << 31) || q_per_seq >= (1ll << 27)) return DSX_EBADSHAPE;
+  if (total >= (1ll << 24)) return DSX_EBADSHAPE;  // a launch has fewer than 2^32 threads
   a.q_per_seq = (int)q_per_seq;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)total), block(256);

@@ -119,6 +119,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     uint64_t beyond;
     if (lens.b0 != 0) load_lens(a, 0, lane, lens);
     while ((beyond = __builtin_amdgcn_ballot_w64(before + lens.upto > place)) == 0) {
+      if (lens.b0 + 64 >= a.n.batch) return;  // (lengths that another stream changed under the kernel)
       before += __builtin_amdgcn_readlane(lens.upto, 63);
       load_lens(a, lens.b0 + 64, lane, lens);
     }
@@ -191,8 +192,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
       const bool bad = id < 0 || id >= r.c.pages;
       pg[hf] = bad ? 0 : id;
       uint32_t ks = ((const uint8_t*)r.c.k_scale)[pg[hf] * r.c.ks_sp + h];
-      const uint32_t vs = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
-      if (bad || vs == 255) ks = 255;  // NaN scores for every row that sees the block
+      uint32_t vs = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
+      if (bad || vs == 255) {  // NaN scores for every row that sees the block, and nothing for the others
+        ks = 255;
+        vs = 127;
+      }
       sc_all |= (ks << (8 * hf)) | (vs << (16 + 8 * hf));
     }
   };
@@ -501,7 +505,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
     pieces = 0;
     if (count > 0) {
       const int n = share_count(total, a.share);
-      const int w0 = share_of(total, n, first), w1 = share_of(total, n, first + count - 1);
+      const int w0 = share_of(total, n, first), w1 = min(share_of(total, n, first + count - 1), n - 1);
       if (w0 == w1) return;  // one workgroup had all of it and wrote the result
       pieces = w1 - w0 + 1;  // the first workgroup's piece begins the unit, the others' continue it
       piece0 = 2 * (int64_t)w0;
@@ -666,7 +670,8 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
   }
   const int per = 16 / plan.ways;
   const int64_t join_wgs = plan.join_units * ((plan.block_rows + per - 1) / per);
-  if (plan.units >= (1ll << 30) || join_wgs >= (1ll << 31)) return DSX_EBADSHAPE;
+  // A launch has fewer than 2^32 threads: 512 a unit (and a few more where the tile form cuts some), 256 a join.
+  if (plan.units >= (1ll << 23) - 4096 || join_wgs >= (1ll << 24)) return DSX_EBADSHAPE;
   AttnArgs a{};
   a.c = c;
   a.n = n;

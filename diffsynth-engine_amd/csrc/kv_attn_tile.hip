@@ -152,8 +152,11 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
           const bool bad = id < 0 || id >= r.c.pages;
           const int64_t page = bad ? 0 : id;
           uint32_t k8 = ((const uint8_t*)r.c.k_scale)[page * r.c.ks_sp + h];
-          const uint32_t v8 = ((const uint8_t*)r.c.v_scale)[page * r.c.vs_sp + h];
-          if (bad || v8 == 255) k8 = 255;  // NaN scores for every row that sees the block
+          uint32_t v8 = ((const uint8_t*)r.c.v_scale)[page * r.c.vs_sp + h];
+          if (bad || v8 == 255) {  // NaN scores for every row that sees the block, and nothing for the others
+            k8 = 255;
+            v8 = 127;
+          }
           ks_all |= k8 << (8 * q);
           vs_all |= v8 << (8 * q);
         }

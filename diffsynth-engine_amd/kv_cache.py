@@ -21,10 +21,26 @@ HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-class KVCache:
+class _Fixed:
+    """Attributes that are set once: the library is handed the addresses and sizes that they had then."""
+
+    def __setattr__(self, name, value):
+        if "_ref" in self.__dict__:
+            raise AttributeError("%s.%s is fixed; make a new one" % (type(self).__name__, name))
+        super().__setattr__(name, value)
+
+
+def _apart(shape, strides, inner: int) -> bool:
+    """Whether blocks of `inner` elements at these (page, head) strides lie apart."""
+    (p, h), (sp, sh) = shape, strides
+    return (p == 1 or sp >= inner) and (h == 1 or sh >= inner) \
+        and (p == 1 or h == 1 or sp >= (h - 1) * sh + inner or sh >= (p - 1) * sp + inner)
+
+
+class KVCache(_Fixed):
     """Codes ``k``, ``v``: (pages, heads, page_size, 128) e4m3, any page and head strides that are multiples of 16, each
     (page, head) block contiguous.  Scales ``k_scale``, ``v_scale``: (pages, heads) e8m0, heads contiguous.  A value is
-    code * scale.  The tensors stay the caller's and are used in place."""
+    code * scale.  The tensors stay the caller's and are used in place; which they are is fixed when the cache is made."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] not in PAGE_SIZES or k.shape != v.shape \
@@ -36,11 +52,15 @@ class KVCache:
                 raise ValueError("KVCache: codes must be float8_e4m3fn, got %s" % t.dtype)
             if t.stride(3) != 1 or t.stride(2) != HEAD_DIM or t.stride(1) % 16 or t.stride(0) % 16 or t.data_ptr() % 16:
                 raise ValueError("KVCache: every (page, head) block must be contiguous and 16-byte aligned")
+            if not _apart(t.shape[:2], t.stride()[:2], t.shape[2] * HEAD_DIM):
+                raise ValueError("KVCache: blocks overlap in memory")
         for t in (k_scale, v_scale):
             if t.dtype != E8M0 or t.shape != k.shape[:2]:
                 raise ValueError("KVCache: scales must be float8_e8m0fnu of shape (pages, heads)")
             if t.shape[1] > 1 and t.stride(1) != 1:
                 raise ValueError("KVCache: the scales of a page must be contiguous")
+            if not _apart(t.shape, t.stride(), 1):
+                raise ValueError("KVCache: scales overlap in memory")
         if any(t.device != k.device for t in (v, k_scale, v_scale)):
             raise ValueError("KVCache: all four tensors must be on one device")
         if k.shape[0] > 0x7fffffff:
@@ -63,7 +83,7 @@ class KVCache:
         return cls(*codes, *scales)
 
 
-class KVPlan:
+class KVPlan(_Fixed):
     """A packed batch: rows [row_start[b], row_start[b + 1]) of q, k and v are the newest tokens of sequence b, which
     has kv_len[b] tokens with them; token t of it is in page page_table[b, t // page_size].
 

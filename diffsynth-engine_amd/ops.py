@@ -656,6 +656,13 @@ def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None)
     return ptr, sr, sh
 
 
+def _kv_apart(name: str, rows: int, heads: int, sr: int, sh: int):
+    """Rows that are written must not overlap (an expanded or overlapping view)."""
+    if (rows > 1 and sr < HEAD_DIM) or (heads > 1 and sh < HEAD_DIM) \
+            or (rows > 1 and heads > 1 and sr < (heads - 1) * sh + HEAD_DIM and sh < (rows - 1) * sr + HEAD_DIM):
+        raise ValueError("%s: its elements overlap in memory" % name)
+
+
 def _kv_device(name: str, cache: KVCache, plan: KVPlan, *tensors) -> int:
     """The one device that everything is on (a number: these calls are short, and device objects take a while)."""
     index = tensors[0].get_device()
@@ -725,6 +732,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
         if q_out is None:
             q_out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
         qop, qo_sr, qo_sh = _kv_rows("kv_append: q_out", q_out, rows, heads)
+        _kv_apart("kv_append: q_out", rows, heads, qo_sr, qo_sh)
     k_norm_w, q_norm_w = _kv_norm_weight(k_norm_w), _kv_norm_weight(q_norm_w)
     rope_sb = rope_rows = 0
     if rope is not None:
@@ -745,7 +753,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     """softmax(q k^T * scale) v of packed rows over the tokens their sequences have in a paged 8-bit cache.
 
     q, out: (rows, heads, 128) bf16, heads a multiple of cache.heads (query head h reads cache head
-    h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8.
+    h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8; out may be q.
     causal: row i of a sequence with r rows sees its first kv_len - r + i + 1 tokens; else all kv_len.  Of these only the
     last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive.
 
@@ -768,6 +776,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     if out is None:
         out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
     op, o_sr, o_sh = _kv_rows("kv_attention: out", out, rows, heads)
+    _kv_apart("kv_attention: out", rows, heads, o_sr, o_sh)
     if not rows:
         return out
     lib = _lib.load()

@@ -392,6 +392,8 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
  * page number outside [0, pages) is not written, and rows that see a token of it become NaN.  dsx_kv_plan_check does the
  * same checks on the host.
  * Rows from row_start[batch] on belong to nobody and are left as they are.
+ * The bounds also limit a launch (DSX_EBADSHAPE beyond): attention to 2^23 - 4096 units of (sequence, cache head, block of
+ * 16, 32 or 256 query rows), an append to 2^24 blocks of (sequence, page that max_rows rows can reach, head).
  */
 typedef struct dsx_kv_cache {
   void* k; void* v;
@@ -445,7 +447,7 @@ int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const ds
  * Query head h reads cache head h / (heads_q / heads); heads_q is a multiple of heads.
  * Softmax and sums in fp32.  q is used as the exact sum of two scaled e4m3 terms (each element to 2^-22 of its row's
  * largest), the weights enter the second product as fp16.  A q row with a non-finite element gives NaN.
- * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned).
+ * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned); out may be q.
  * workspace: dsx_kv_attn_workspace_bytes(...) bytes, 16-byte aligned, lets the key range be split over the compute units
  * and the pieces be joined by a second launch; NULL: never split.  Calls that share a workspace must not overlap.
  */

@@ -673,3 +673,58 @@ def test_scores_that_move_the_reference(dev, page, rows, shape):
         got = c.attend(causal=causal)
         want, size = c.want(causal=causal)
         close(got, want, 2 * size, c.starts[-1])
+
+
+@pytest.mark.parametrize("rows,lens,window", [([5], [200], 0), ([40], [200], 0), ([150, 3], [200, 150], 40), ([3] * 4, [2000] * 4, 0)])
+def test_a_scale_of_nan_reaches_only_rows_that_see_its_block(dev, rows, lens, window):
+    for page in (16, 64):
+        c = Case(dev, rows, lens, group=2, page=page, seed=page)
+        clean = c.attend(window=window)
+        for at in (lens[0] - 2, lens[0] - rows[0]):  # the block of this token
+            for scale in (c.cache.k_scale, c.cache.v_scale):
+                raw = scale.view(torch.uint8)
+                old = raw[c.table[0][at // page], 1].clone()
+                raw[c.table[0][at // page], 1] = 255
+                got = c.attend(window=window)
+                raw[c.table[0][at // page], 1] = old
+                first, last = at // page * page, min(at // page * page + page, lens[0]) - 1  # the block's tokens
+                pos = torch.arange(lens[0] - rows[0], lens[0])
+                sees = (pos >= first) & ((pos - window < last) if window else torch.ones_like(pos, dtype=torch.bool))
+                mine = torch.zeros(c.total, 4, dtype=torch.bool)
+                mine[:rows[0], 2:] = sees[:, None]
+                mine = mine.to(dev)
+                assert got[mine].isnan().all() and torch.equal(got[~mine], clean[~mine]), (page, at)
+
+
+def test_no_tokens_at_all(dev):
+    for rows in ([1, 2], [20, 3], [300, 1]):
+        c = Case(dev, rows, [0, 0], group=2, seed=1)
+        for bound in (0, 4096):
+            from diffsynth_engine_amd import kv_cache
+
+            plan = kv_cache.KVPlan(torch.zeros(2, 64, dtype=torch.int32, device=dev), c.plan.row_start, c.plan.kv_len,
+                                   max_rows=max(rows), max_kv_len=bound)
+            c.plan = plan
+            assert (c.attend() == 0).all() and (c.attend(causal=False, window=3) == 0).all()
+
+
+@pytest.mark.parametrize("rows,lens", [([1, 3], [3000, 50]), ([30], [700]), ([600], [900])])
+def test_out_may_be_q(dev, rows, lens):
+    c = Case(dev, rows, lens, group=3, seed=rows[0])
+    q, want = c.q.to(dev), c.attend()
+    assert c.attend(q=q, out=q) is q and torch.equal(q, want)
+
+
+def test_outputs_that_overlap_are_refused(dev):
+    from diffsynth_engine_amd import ops
+
+    c = Case(dev, [2, 3], [40, 50], group=2, page=16, seed=5)
+    q, k, v = c.q.to(dev), c.k.to(dev), c.v.to(dev)
+    flat = torch.empty(5 * 9 * 128, dtype=BF, device=dev)
+    for bad in (q[:1].expand(5, -1, -1), q[:, :1].expand(-1, 4, -1), flat.as_strided((5, 4, 128), (256, 128, 1))):
+        with pytest.raises(ValueError):
+            ops.kv_attention(q, c.cache, c.plan, out=bad)
+        with pytest.raises(ValueError):
+            ops.kv_append(k, v, c.cache, c.plan, q=q, q_out=bad)
+    out = flat.view(5, 9, 128)[:, 1:8:2]  # every other head of a wider buffer
+    assert torch.equal(ops.kv_attention(q, c.cache, c.plan, out=out), ops.kv_attention(q, c.cache, c.plan))

@@ -68,6 +68,24 @@ def test_cache_refuses_what_does_not_fit():
     assert KVCache(both[:, 0], both[:, 1], c.k_scale, c.v_scale)._c.k_sp == 2 * 2 * 16 * 128
 
 
+def test_cache_and_plan_are_fixed_and_blocks_lie_apart():
+    from diffsynth_engine_amd.kv_cache import KVCache
+
+    c, plan = _cache(), _plan()
+    for thing, name in ((c, "k"), (c, "v_scale"), (c, "page_size"), (plan, "kv_len"), (plan, "max_kv_len")):
+        with pytest.raises(AttributeError):
+            setattr(thing, name, getattr(thing, name))
+    k, s = c.k.view(torch.uint8), c.k_scale.view(torch.uint8)
+    for codes, scales in ((k[:1].expand(4, -1, -1, -1), s), (k[:, :1].expand(-1, 2, -1, -1), s), (k, s[:1].expand(4, -1)),
+                          (k.as_strided((4, 2, 16, 128), (2048, 2048, 128, 1)), s), (k, s.as_strided((4, 2), (1, 1)))):
+        with pytest.raises(ValueError):
+            KVCache(codes.view(F8), c.v, scales.view(E8), c.v_scale)
+    heads_outside = k.transpose(0, 1).contiguous().transpose(0, 1).view(F8)  # (pages, heads) stored the other way round
+    assert KVCache(heads_outside, c.v, c.k_scale, c.v_scale)._c.k_sp == 2048
+    every_other = torch.zeros(4, 3, 16, 128, dtype=torch.uint8)[:, ::2].view(F8)
+    assert KVCache(every_other, c.v, c.k_scale, c.v_scale)._c.k_sh == 4096
+
+
 def test_plan_refuses_what_does_not_fit():
     from diffsynth_engine_amd.kv_cache import KVPlan
 
@@ -180,6 +198,12 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
                    (dict(norm_eps=math.nan), _lib.DSX_EBADSHAPE), (dict(rope=at, rope_rows=31), _lib.DSX_EBADSHAPE),
                    (dict(rope=at, rope_rows=32, rope_sb=128), _lib.DSX_EBADSHAPE)):
         assert append(**kw) == rc, kw
+    # bounds that no launch could cover
+    large = changed(plan._c, batch=1 << 23, max_rows=4)
+    assert attn(n=large) == _lib.DSX_EBADSHAPE and append(n=large) == _lib.DSX_EBADSHAPE
+    rows = changed(plan._c, batch=1 << 12, max_rows=1 << 20, max_kv_len=1 << 20, table_pages=1 << 16, table_sb=1 << 16)
+    assert append(n=rows, total_rows=1 << 20) == _lib.DSX_EBADSHAPE
+    assert attn(n=rows, total_rows=1 << 20) == _lib.DSX_EBADSHAPE
 
 
 def test_oracle_rounding_against_torch_and_known_answers():
