@@ -83,6 +83,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   const dsx_kv_append_params& p = a.p;
   const int tid = threadIdx.x, ln = tid & 15, grp = tid >> 4;
   __shared__ uint32_t smax[4];
+  asm volatile("" ::"s"(c.k), "s"(n.row_start), "s"(p.k), "s"(p.q_norm_w), "s"(p.total_rows), "s"(a.q_begin));
 
   if ((int64_t)blockIdx.x >= a.q_begin) {
     const unsigned u = blockIdx.x - (unsigned)a.q_begin;

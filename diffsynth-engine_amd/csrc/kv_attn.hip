@@ -75,11 +75,17 @@ __device__ __forceinline__ int share_of(int total, int n, int x) {  // whose run
   return (int)((((uint64_t)x + 1) * n - 1) / (uint64_t)total);
 }
 
-template <int NQ>  // 16-row columns of query rows
+template <int NQ, bool SHARE>  // 16-row columns of query rows; even shares (a.share) or a.splits pieces of every unit
 __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
-  const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = uniform(threadIdx.x >> 6);
+  // The lane's number, anew where it is asked for: sums of it for the end of the kernel would be made at its beginning and
+  // held, or spilled, across the tiles.
+  auto this_lane = [&]() __attribute__((always_inline)) {
+    int x = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   // Halves of the waves' results, lane after lane, then (row, element) by wave: never both at once.
   __shared__ union {
     struct {
@@ -92,11 +98,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     } row;
   } sm;
 
+  // All of the argument block at once: five cache lines, which would be met one after another.
+  asm volatile("" ::"s"(a.c.k), "s"(a.n.row_start), "s"(a.p.q), "s"(a.p.total_rows), "s"(a.part_o));
+
   // This workgroup's tiles among all of them, as head and place in the head (one whole unit: nothing to look up).
   int h = 0, place = 0, left = 1, head_tiles = 1;
   Lens lens;
-  if (a.share) {
-    head_tiles = head_sum(a, lane, lens);
+  if constexpr (SHARE) {
+    head_tiles = head_sum(a, this_lane(), lens);
     const int total = head_tiles * c.heads;
     if (total == 0) return;
     const int n = share_count(total, a.share);
@@ -107,10 +116,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     place -= h * head_tiles;
   }
   for (bool again = false; left > 0; again = true) {
+  const int lane = this_lane(), n16 = lane & 15, g4 = lane >> 4;
   // ---- the next segment: a whole unit or a part of one
   int b, qb = 0, skip = 0, count = 0x3fffffff, piece = -1;  // piece: where a part's result goes
   KvSeq s;
-  if (a.share) {
+  if constexpr (SHARE) {
     if (place == head_tiles) {
       place = 0;
       ++h;
@@ -136,10 +146,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     place += count;
     left -= count;
   } else {
-    kv_unit(a, blockIdx.x / a.splits, b, h, qb);
+    kv_unit(a, blockIdx.x / (unsigned)a.splits, b, h, qb);
     s = kv_seq(a.n, b, a.p.total_rows);
     left = 0;
   }
+  // (one value each for the whole wave, which divisions and loads leave in vector registers)
+  b = uniform(b);
+  h = uniform(h);
+  qb = uniform(qb);
+  s = {uniform(s.row0), uniform(s.rows), uniform(s.kv), uniform((int)s.ok) != 0};
   const int packed = s.rows * a.group;
   const int pr0 = qb * 16 * NQ;
   if (pr0 >= packed) return;
@@ -152,9 +167,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   kv_row_span(s.kv, s.rows, row_hi, a.p.causal, a.p.window, lo_last, hi_last);
   const int tile_end = (hi_last + kTileKeys - 1) / kTileKeys;
   int t_begin = lo_first / kTileKeys;
-  if (a.splits > 1) {
+  if (!SHARE && a.splits > 1) {
     count = (max(tile_end - t_begin, 0) + a.splits - 1) / a.splits;
-    skip = (int)(blockIdx.x % a.splits) * count;
+    skip = (int)(blockIdx.x % (unsigned)a.splits) * count;
     piece = blockIdx.x;
   }
   t_begin += skip;
@@ -173,7 +188,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 
   const uint8_t* kbase = (const uint8_t*)c.k + (int64_t)h * c.k_sh;
   const uint8_t* vbase = (const uint8_t*)c.v + (int64_t)h * c.v_sh;
-  const int koff = n16 * kKvDim + 16 * g4, voff = 4 * g4 * kKvDim + 8 * n16;
+  const uint32_t koff = n16 * kKvDim + 16 * g4, voff = 4 * g4 * kKvDim + 8 * n16;
   const int page_mask = c.page_size - 1;
 
   // Page numbers and scales of 64 of the wave's tiles, one tile per lane: two dependent loads per 64 tiles instead of two
@@ -181,28 +196,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   // loaded for them is not used.
   int pg[2] = {0, 0}, pg_at = -1;
   uint32_t sc_all = 0;
-  auto preload = [&](int chunk) __attribute__((always_inline)) {
+  uint32_t ks[2], vs[2];  // scale bytes on their way
+  bool bad[2];
+  auto ask_pages = [&](int chunk) __attribute__((always_inline)) {
     const AttnArgs& r = args_again();
     pg_at = chunk;
-    sc_all = 0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int key = min((t_begin + wave + kWaves * (64 * chunk + lane)) * kTileKeys + 16 * hf, hi_last - 1);
-      const int id = r.n.page_table[b * r.n.table_sb + (key >> r.page_shift)];
-      const bool bad = id < 0 || id >= r.c.pages;
-      pg[hf] = bad ? 0 : id;
-      uint32_t ks = ((const uint8_t*)r.c.k_scale)[pg[hf] * r.c.ks_sp + h];
-      uint32_t vs = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
-      if (bad || vs == 255) {  // NaN scores for every row that sees the block, and nothing for the others
-        ks = 255;
-        vs = 127;
-      }
-      sc_all |= (ks << (8 * hf)) | (vs << (16 + 8 * hf));
+      pg[hf] = r.n.page_table[b * r.n.table_sb + (key >> r.page_shift)];
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      bad[hf] = pg[hf] < 0 || pg[hf] >= r.c.pages;
+      pg[hf] = bad[hf] ? 0 : pg[hf];
+      ks[hf] = ((const uint8_t*)r.c.k_scale)[pg[hf] * r.c.ks_sp + h];
+      vs[hf] = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
     }
   };
-  auto load_tile = [&](int i, TileRegs& r) __attribute__((always_inline)) -> uint32_t {  // returns its scales
-    if ((i >> 6) != pg_at) preload(i >> 6);
+  auto take_scales = [&]() __attribute__((always_inline)) {
+    sc_all = 0;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      // (no scale: NaN scores for every row that sees the block, and nothing for the others)
+      const bool none = bad[hf] || vs[hf] == 255;
+      sc_all |= ((none ? 255u : ks[hf]) << (8 * hf)) | ((none ? 127u : vs[hf]) << (16 + 8 * hf));
+    }
+  };
+  auto scales_at = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)sc_all, i & 63); };
+  auto load_codes = [&](int i, TileRegs& r) __attribute__((always_inline)) {
     const int key = (t_begin + wave + kWaves * i) * kTileKeys;
+    uint32_t ko = koff, vo = voff;
+    asm volatile("" : "+v"(ko), "+v"(vo));  // (32-bit offsets to a scalar base; widened outside, they would be 64-bit sums)
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int64_t page = __builtin_amdgcn_readlane(pg[hf], i & 63);
@@ -210,11 +235,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
       const uint8_t* kp = kbase + page * c.k_sp + tok * kKvDim;
       const uint8_t* vp = vbase + page * c.v_sp + tok * kKvDim;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) r.k[hf][w] = *reinterpret_cast<const u32x4*>(kp + koff + 64 * w);
+      for (int w = 0; w < 2; ++w) r.k[hf][w] = *reinterpret_cast<const u32x4*>(kp + ko + 64 * w);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) r.v[hf][t] = *reinterpret_cast<const u32x2*>(vp + voff + t * kKvDim);
+      for (int t = 0; t < 4; ++t) r.v[hf][t] = *reinterpret_cast<const u32x2*>(vp + vo + t * kKvDim);
     }
-    return (uint32_t)__builtin_amdgcn_readlane((int)sc_all, i & 63);
+  };
+  auto load_tile = [&](int i, TileRegs& r) __attribute__((always_inline)) -> uint32_t {  // returns its scales
+    if ((i >> 6) != pg_at) {
+      ask_pages(i >> 6);
+      take_scales();
+    }
+    load_codes(i, r);
+    return scales_at(i);
   };
 
   // ---- tiles in flight: kRing - 1 of the inner ones, and in front of them the first that has to be masked (the last of a
@@ -223,10 +255,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   TileRegs ring[kRing];
   uint32_t sc[kRing];
   const int first_masked = in_lo > 0 ? 0 : in_hi;
-  if (first_masked < tiles) sc[kRing - 1] = load_tile(first_masked, ring[kRing - 1]);
+  const int chunk = (first_masked < tiles ? first_masked : in_lo) >> 6;
+  const bool near = (in_lo + kRing - 2) >> 6 == chunk;
+  if (tiles > 0) {
+    // (the first codes are asked for along with the scales, not behind them)
+    ask_pages(chunk);
+    if (first_masked < tiles) load_codes(first_masked, ring[kRing - 1]);
 #pragma unroll
-  for (int r = 0; r < kRing - 1; ++r)
-    if (in_lo + r < in_hi) sc[r] = load_tile(in_lo + r, ring[r]);
+    for (int r = 0; r < kRing - 1; ++r)
+      if (near && in_lo + r < in_hi) load_codes(in_lo + r, ring[r]);
+  }
   __builtin_amdgcn_sched_barrier(0);
 
   QFrag qf[NQ];
@@ -240,6 +278,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  __builtin_amdgcn_sched_barrier(0);
+  if (tiles > 0) {
+    take_scales();
+    sc[kRing - 1] = scales_at(first_masked);
+#pragma unroll
+    for (int r = 0; r < kRing - 1; ++r)
+      if (in_lo + r < in_hi) sc[r] = near ? scales_at(in_lo + r) : load_tile(in_lo + r, ring[r]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   const float cs = a.p.softmax_scale * kLog2e;
 
   auto compute = [&](auto masked, int i, TileRegs& r, uint32_t sc) __attribute__((always_inline)) {
@@ -401,9 +448,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 
   // ---- the waves' results join in LDS, one 16-row column at a time: the upper half of the waves hands its lanes to the
   //      lower half's, the rest is joined by (row, 4 elements) per thread
-  const int d0 = (tid & 31) * 4;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
+    const int lane = this_lane(), n16 = lane & 15, g4 = lane >> 4, d0 = (lane & 31) * 4;
     if (q) __syncthreads();
     if (wave >= kWaves / 2) {
       const int w = wave - kWaves / 2;
@@ -440,7 +487,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
               f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
     }
     __syncthreads();
-    for (int row16 = tid >> 5; row16 < 16; row16 += 2 * kWaves) {
+    static_assert(2 * kWaves == 16, "half a wave to a row");
+    const int row16 = 2 * wave + (lane >> 5);
+    {
       float m = -INFINITY, l = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -479,12 +528,13 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
   const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
   __shared__ float sm_o[16][kKvDim + 4];
   __shared__ float sm_m[16], sm_l[16];
+  asm volatile("" ::"s"(a.n.row_start), "s"(a.p.out), "s"(a.p.total_rows), "s"(a.part_o));
   const int per = 16 / ways, slot = grp / ways, way = grp % ways;
   const int blocks = (a.block_rows + per - 1) / per;
-  const int64_t cut = blockIdx.x / blocks;  // the unit, counted from the first that is cut
-  const int r = (int)(blockIdx.x % blocks) * per + slot;
+  const int64_t cut = blockIdx.x / (unsigned)blocks;  // the unit, counted from the first that is cut
+  const int r = (int)(blockIdx.x % (unsigned)blocks) * per + slot;
   int b, h, qb;
-  kv_unit(a, a.first_split + cut, b, h, qb);
+  kv_unit(a, (uint32_t)(a.first_split + cut), b, h, qb);
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
   const int pr = qb * a.block_rows + r;
   const bool live = r < a.block_rows && pr < s.rows * a.group;
@@ -514,7 +564,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
     }
   }
   float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int t = way; live && t < pieces; t += ways) {
+  for (int t = way; r < a.block_rows && t < pieces; t += ways) {  // (dead rows too: a piece has all of them)
     const int64_t at = (piece0 + (int64_t)t * step + (t == 0 ? odd : 0)) * a.block_rows + r;
     const float mt = a.part_ml[2 * at], lt = a.part_ml[2 * at + 1];
     const f32x4 lo = *reinterpret_cast<const f32x4*>(a.part_o + at * kKvDim + d0);
@@ -632,7 +682,10 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
 
 template <int NQ>
 void launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
-  kv_stream_kernel<NQ><<<dim3((unsigned)(a.share ? a.share : units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
+  if (a.share)
+    kv_stream_kernel<NQ, true><<<dim3((unsigned)a.share), dim3(64 * kWaves), 0, st>>>(a);
+  else
+    kv_stream_kernel<NQ, false><<<dim3((unsigned)(units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
 }
 
 }  // namespace

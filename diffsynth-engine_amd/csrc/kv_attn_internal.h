@@ -26,12 +26,12 @@ struct AttnArgs {
 
 // Unit number -> (sequence, cache head, query block).  Sequences inside heads: runs of units (the tile form gives each XCD
 // one) then hold all sequences alike, long and short.  Causal blocks come last first: they are the longest.
-__device__ __forceinline__ void kv_unit(const AttnArgs& a, int64_t unit, int& b, int& h, int& qb) {
-  qb = (int)(unit % a.nqb);
+__device__ __forceinline__ void kv_unit(const AttnArgs& a, uint32_t unit, int& b, int& h, int& qb) {
+  qb = (int)(unit % (uint32_t)a.nqb);
   if (a.p.causal) qb = a.nqb - 1 - qb;
-  unit /= a.nqb;
-  b = (int)(unit % a.n.batch);
-  h = (int)(unit / a.n.batch);
+  unit /= (uint32_t)a.nqb;
+  b = (int)(unit % (uint32_t)a.n.batch);
+  h = (int)(unit / (uint32_t)a.n.batch);
 }
 
 // Inclusive sum over the lanes of a wave: six adds, each fed by the row shifts and broadcasts of the vector unit.
@@ -48,6 +48,8 @@ __device__ __forceinline__ int wave_scan(int v) {
   v = dpp_add<0x143, 0xc>(v);  // row_bcast31 into rows 2 and 3
   return v;
 }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ float quad_max(float v) {  // over the four lanes n, n + 16, n + 32, n + 48
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -66,14 +66,14 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     if (unit >= a.first_split) return;
   } else {
     const unsigned j = blockIdx.x - whole8;
-    const int64_t piece = (int64_t)(j & 7) * (cut8 >> 3) + (j >> 3);
+    const unsigned piece = (j & 7) * (unsigned)(cut8 >> 3) + (j >> 3);
     if (piece >= (units - a.first_split) * a.splits) return;
-    unit = a.first_split + piece / a.splits;
-    split = (int)(piece % a.splits);
+    unit = a.first_split + piece / (unsigned)a.splits;
+    split = (int)(piece % (unsigned)a.splits);
     splits = a.splits;
   }
   int b, h, qb;
-  kv_unit(a, unit, b, h, qb);
+  kv_unit(a, (uint32_t)unit, b, h, qb);
   b = __builtin_amdgcn_readfirstlane(b);
   h = __builtin_amdgcn_readfirstlane(h);
   qb = __builtin_amdgcn_readfirstlane(qb);

@@ -16,7 +16,11 @@ struct KvSeq {
   bool ok;
 };
 __host__ __device__ inline KvSeq kv_seq(const dsx_kv_batch& n, int b, int64_t total_rows) {
-  const int r0 = n.row_start[b], r1 = n.row_start[b + 1], kv = n.kv_len[b];
+  const int r0 = n.row_start[b], r1 = n.row_start[b + 1];
+  int kv = n.kv_len[b];
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(kv));  // (loaded along with the rows, not behind a look at them: a trip to memory less)
+#endif
   if (r0 < 0 || r1 < r0 || r1 > total_rows) return {0, 0, 0, false};
   const bool ok = r1 - r0 <= n.max_rows && kv >= 0 && kv <= n.max_kv_len;
   return {r0, r1 - r0 <= n.max_rows ? r1 - r0 : n.max_rows, ok ? kv : 0, ok};
