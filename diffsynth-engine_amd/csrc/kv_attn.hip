@@ -40,6 +40,11 @@ struct TileRegs {
 
 constexpr int kWaves = 8;
 
+struct StreamLds {  // the waves' results
+  float o[kWaves][16][kKvDim + 4];
+  float m[kWaves][16], l[kWaves][16];
+};
+
 // ---- Equal shares.  The tiles of all units lie behind one another, head by head and sequence by sequence, and are dealt
 // to `share` workgroups in equal runs whatever the sequences' lengths (which only the device knows): a run may end inside
 // a unit, and then both sides leave partial results.  Every wave sums the lengths for itself, a sequence per lane.
@@ -86,18 +91,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     asm volatile("" : "+v"(x));
     return x;
   };
-  // Halves of the waves' results, lane after lane, then (row, element) by wave: never both at once.
-  __shared__ union {
-    struct {
-      f32x4 o[kWaves / 2][8][64];
-      float m[kWaves / 2][64], l[kWaves / 2][64];
-    } half;
-    struct {
-      float o[kWaves / 2][16][kKvDim + 4];
-      float m[kWaves / 2][16], l[kWaves / 2][16];
-    } row;
-  } sm;
-
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  StreamLds* sm = reinterpret_cast<StreamLds*>(smem);
   // All of the argument block at once: five cache lines, which would be met one after another.
   asm volatile("" ::"s"(a.c.k), "s"(a.n.row_start), "s"(a.p.q), "s"(a.p.total_rows), "s"(a.part_o));
 
@@ -446,59 +441,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     }
   }
 
-  // ---- the waves' results join in LDS, one 16-row column at a time: the upper half of the waves hands its lanes to the
-  //      lower half's, the rest is joined by (row, 4 elements) per thread
+  // ---- the waves' results join in LDS, one 16-row column at a time; half a wave then takes a row
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const int lane = this_lane(), n16 = lane & 15, g4 = lane >> 4, d0 = (lane & 31) * 4;
+    const int live = packed - pr0 - q * 16;  // rows behind the last one are worth no trip
     if (q) __syncthreads();
-    if (wave >= kWaves / 2) {
-      const int w = wave - kWaves / 2;
-      sm.half.m[w][lane] = m_run[q];
-      sm.half.l[w][lane] = l_run[q];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sm.half.o[w][i][lane] = o[q][i];
-    }
-    __syncthreads();
-    if (wave < kWaves / 2) {
-      const float mb = sm.half.m[wave][lane], m = fmaxf(m_run[q], mb);
-      const float fa = join_factor(m_run[q], m), fb = join_factor(mb, m);
-      m_run[q] = m;
-      l_run[q] = l_run[q] * fa + sm.half.l[wave][lane] * fb;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const f32x4 x = sm.half.o[wave][i][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[q][i][e] = o[q][i][e] * fa + x[e] * fb;
-      }
-    }
-    __syncthreads();
-    if (wave < kWaves / 2) {
-      const float l = quad_sum(l_run[q]);
+    const float l_row = quad_sum(l_run[q]);
+    if (n16 < live) {
       if (g4 == 0) {
-        sm.row.m[wave][n16] = m_run[q];
-        sm.row.l[wave][n16] = l;
+        sm->m[wave][n16] = m_run[q];
+        sm->l[wave][n16] = l_row;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < 8; i += 4)
-          *reinterpret_cast<f32x4*>(&sm.row.o[wave][n16][32 * g4 + 8 * r + i]) =
+          *reinterpret_cast<f32x4*>(&sm->o[wave][n16][32 * g4 + 8 * r + i]) =
               f32x4{o[q][i][r], o[q][i + 1][r], o[q][i + 2][r], o[q][i + 3][r]};
     }
     __syncthreads();
     static_assert(2 * kWaves == 16, "half a wave to a row");
     const int row16 = 2 * wave + (lane >> 5);
-    {
+    if (row16 < live) {
       float m = -INFINITY, l = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kWaves / 2; ++w) m = fmaxf(m, sm.row.m[w][row16]);
+      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sm->m[w][row16]);
 #pragma unroll
-      for (int w = 0; w < kWaves / 2; ++w) {
-        const float f = join_factor(sm.row.m[w][row16], m);
-        l = __builtin_fmaf(sm.row.l[w][row16], f, l);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.row.o[w][row16][d0]);
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = join_factor(sm->m[w][row16], m);
+        l = __builtin_fmaf(sm->l[w][row16], f, l);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&sm->o[w][row16][d0]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
       }
@@ -510,7 +484,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
           a.part_ml[2 * at] = m;
           a.part_ml[2 * at + 1] = l;
         }
-      } else if (pr < packed) {
+      } else {
         const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
         const u32x2 w = {pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
         const int row = pr / a.group, hh = h * a.group + pr % a.group;
@@ -680,12 +654,21 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   return r;
 }
 
+template <int NQ, bool SHARE>
+int launch_stream(const AttnArgs& a, unsigned workgroups, hipStream_t st) {
+  static PerDeviceOnce attr_once;
+  const int rc = per_device_once(attr_once, [](int) {
+    return hipFuncSetAttribute((const void*)kv_stream_kernel<NQ, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)sizeof(StreamLds)) == hipSuccess ? (int)DSX_OK : (int)DSX_ELAUNCH;
+  });
+  if (rc != DSX_OK) return rc;
+  kv_stream_kernel<NQ, SHARE><<<dim3(workgroups), dim3(64 * kWaves), sizeof(StreamLds), st>>>(a);
+  return DSX_OK;
+}
 template <int NQ>
-void launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
-  if (a.share)
-    kv_stream_kernel<NQ, true><<<dim3((unsigned)a.share), dim3(64 * kWaves), 0, st>>>(a);
-  else
-    kv_stream_kernel<NQ, false><<<dim3((unsigned)(units * a.splits)), dim3(64 * kWaves), 0, st>>>(a);
+int launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
+  return a.share ? launch_stream<NQ, true>(a, (unsigned)a.share, st)
+                 : launch_stream<NQ, false>(a, (unsigned)(units * a.splits), st);
 }
 
 }  // namespace
@@ -741,14 +724,10 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
     a.part_ml = a.part_o + plan.ws_bytes / (4 * (kKvDim + 2)) * kKvDim;
   }
   hipStream_t st = (hipStream_t)stream;
-  if (plan.nq == 1) {
-    launch_stream<1>(a, plan.units, st);
-  } else if (plan.nq == 2) {
-    launch_stream<2>(a, plan.units, st);
-  } else {
-    const int trc = launch_kv_tile(a, plan.units, st);
-    if (trc != DSX_OK) return trc;
-  }
+  const int lrc = plan.nq == 1   ? launch_stream<1>(a, plan.units, st)
+                  : plan.nq == 2 ? launch_stream<2>(a, plan.units, st)
+                                 : launch_kv_tile(a, plan.units, st);
+  if (lrc != DSX_OK) return lrc;
   if (hipGetLastError() != hipSuccess) return DSX_ELAUNCH;
   if (join_wgs > 0) kv_join_kernel<<<dim3((unsigned)join_wgs), dim3(256), 0, st>>>(a, plan.ways);
   return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;

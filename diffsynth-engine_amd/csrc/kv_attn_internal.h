@@ -75,40 +75,10 @@ __device__ __forceinline__ float join_factor(float m, float to) {
   return m == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - to);
 }
 
-// q row -> two e4m3 terms and their e8m0 scales.  x: the lane's 32 elements; the four lanes of a row share the exponent.
 struct QFrag {
   i32x8 hi, lo;
   int s_hi, s_lo;
 };
-__device__ __forceinline__ void split_q(const float (&x)[32], QFrag& f) {
-  float amax = 0.f;
-  bool odd = false;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    amax = fmaxf(amax, fabsf(x[j]));
-    odd |= !(fabsf(x[j]) < INFINITY);
-  }
-  amax = quad_max(odd ? INFINITY : amax);
-  const uint32_t bits = __float_as_uint(amax);
-  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  e = max(e, -110);
-  const bool bad = !(amax < INFINITY);
-  if (bad) e = 0;
-  const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, a normal number for e in [-110, 120]
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    float y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = bad ? 0.f : x[4 * w + j] * down;
-    const uint32_t hi = pack_e4m3x4_inrange(y[0], y[1], y[2], y[3]);
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
-    f.hi[w] = (int)hi;
-    f.lo[w] = (int)pack_e4m3x4_inrange(16.f * (y[0] - a[0]), 16.f * (y[1] - a[1]), 16.f * (y[2] - b[0]),
-                                       16.f * (y[3] - b[1]));
-  }
-  f.s_hi = bad ? 255 : 127 + e;
-  f.s_lo = bad ? 255 : 127 + e - 4;
-}
 
 // Packed query row `pr` of a cache head: its span and its operand (the lane's elements 16g .. +15 and 64 + 16g .. +15).
 struct QRaw {
@@ -122,16 +92,40 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const KvSeq& s, int h,
 #pragma unroll
   for (int w = 0; w < 4; ++w) raw.w[w] = *reinterpret_cast<const u32x4*>(src + 64 * (w >> 1) + 8 * (w & 1));
 }
+// q row -> two e4m3 terms and their e8m0 scales; the four lanes of a row share the exponent.  The converter divides by a
+// power of two before it rounds, and multiplies on the way back.
 __device__ __forceinline__ void split_q(const QRaw& raw, QFrag& f) {
-  float x[32];
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};
 #pragma unroll
   for (int w = 0; w < 4; ++w)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[8 * w + 2 * j] = bf16_lo(raw.w[w][j]);
-      x[8 * w + 2 * j + 1] = bf16_hi(raw.w[w][j]);
-    }
-  split_q(x, f);
+    for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw.w[w][j] & 0x7fff7fffu));
+  const uint32_t most = max((uint32_t)top[0], (uint32_t)top[1]);
+  const float amax = quad_max(__uint_as_float(min(most, 0x7f80u) << 16));  // infinity if any element is not finite
+  const uint32_t bits = __float_as_uint(amax);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = max(e, -110);
+  const bool bad = !(amax < INFINITY);  // a scale of NaN: whatever the codes are, the scores are NaN
+  if (bad) e = 0;
+  const float up_hi = __uint_as_float((uint32_t)(127 + e) << 23), up_lo = __uint_as_float((uint32_t)(123 + e) << 23);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const uint32_t r0 = raw.w[w >> 1][2 * (w & 1)], r1 = raw.w[w >> 1][2 * (w & 1) + 1];
+    const float x[4] = {bf16_lo(r0), bf16_hi(r0), bf16_lo(r1), bf16_hi(r1)};
+    s16x2 hi = {0, 0}, lo = {0, 0};
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[0], x[1], up_hi, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[2], x[3], up_hi, true);
+    f.hi[w] = __builtin_bit_cast(int, hi);
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(f.hi[w], up_hi, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(f.hi[w], up_hi, true);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0] - a[0], x[1] - a[1], up_lo, false);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2] - b[0], x[3] - b[1], up_lo, true);
+    f.lo[w] = __builtin_bit_cast(int, lo);
+  }
+  f.s_hi = bad ? 255 : 127 + e;
+  f.s_lo = bad ? 255 : 123 + e;
 }
 
 // A kernel's own argument block, read again where it is needed: what only the rare paths use would otherwise sit in
