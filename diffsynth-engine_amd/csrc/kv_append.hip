@@ -22,7 +22,8 @@ struct AppendArgs {
   int page_shift;
   int blocks_per_seq;  // pages that max_rows rows can reach
   int64_t q_begin;     // first workgroup of the q part
-  int q_per_seq;
+  int q_per_seq, q_per_row;  // workgroups a sequence, kQHeads heads a row
+  Divisor by_heads, by_blocks, by_q_per_seq, by_q_per_row;
 };
 
 __device__ __forceinline__ float row16_sum(float v) {  // over the 16 lanes of a token
@@ -87,17 +88,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 
   if ((int64_t)blockIdx.x >= a.q_begin) {
     const unsigned u = blockIdx.x - (unsigned)a.q_begin;
-    const int b = (int)(u / (unsigned)a.q_per_seq), chunk = (int)(u % (unsigned)a.q_per_seq);
+    const int b = a.by_q_per_seq(u), chunk = (int)u - b * a.q_per_seq;
     const KvSeq s = kv_seq(n, b, p.total_rows);
     if (!s.ok || s.kv < s.rows) return;
-    const int per_row = (p.heads_q + kQHeads - 1) / kQHeads;
-    const int at = chunk * 16 + grp, row = at / per_row, h0 = at % per_row * kQHeads;
+    const int at = chunk * 16 + grp, row = a.by_q_per_row(at), h0 = (at - row * a.q_per_row) * kQHeads;
     if (row >= s.rows) return;
-    const uint16_t* src = (const uint16_t*)p.q + (int64_t)(s.row0 + row) * p.q_sr + 8 * ln;
-    uint16_t* dst = (uint16_t*)p.q_out + (int64_t)(s.row0 + row) * p.qo_sr + 8 * ln;
+    const uint16_t* src = (const uint16_t*)p.q + times(s.row0 + row, p.q_sr) + 8 * ln;
+    uint16_t* dst = (uint16_t*)p.q_out + times(s.row0 + row, p.qo_sr) + 8 * ln;
     float x[kQHeads][8], g[8], cs[8];
 #pragma unroll
-    for (int i = 0; i < kQHeads; ++i) load8(src + min(h0 + i, p.heads_q - 1) * p.q_sh, x[i]);
+    for (int i = 0; i < kQHeads; ++i) load8(src + times(min(h0 + i, p.heads_q - 1), p.q_sh), x[i]);
     if (p.q_norm_w) load8((const uint16_t*)p.q_norm_w + 8 * ln, g);
     if (p.rope) load_turn(p.rope + b * p.rope_sb + (int64_t)(s.kv - s.rows + row) * kKvDim, ln, cs);
 #pragma unroll
@@ -107,18 +107,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
       u32x4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[i][2 * j], x[i][2 * j + 1]);
-      if (h0 + i < p.heads_q) *reinterpret_cast<u32x4*>(dst + (h0 + i) * p.qo_sh) = w;
+      if (h0 + i < p.heads_q) *reinterpret_cast<u32x4*>(dst + times(h0 + i, p.qo_sh)) = w;
     }
     return;
   }
 
   // ---- one (page, head) block of K or V
-  unsigned u = blockIdx.x;
-  const int h = (int)(u % c.heads);
-  u /= c.heads;
+  const unsigned u = a.by_heads(blockIdx.x);
+  const int h = (int)(blockIdx.x - u * c.heads);
   const bool is_v = u & 1;
-  u >>= 1;
-  const int j = (int)(u % a.blocks_per_seq), b = (int)(u / a.blocks_per_seq);
+  const int b = a.by_blocks(u >> 1), j = (int)(u >> 1) - b * a.blocks_per_seq;
   const KvSeq s = kv_seq(n, b, p.total_rows);
   if (!s.ok || s.kv < s.rows) return;
   const int first = s.kv - s.rows;  // the first appended token
@@ -126,11 +124,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   const int pi = (first >> a.page_shift) + j;
   const int base = pi << a.page_shift;  // the block's first token
   if (base >= s.kv || s.rows == 0) return;
-  const int id = n.page_table[b * n.table_sb + pi];
+  const int id = n.page_table[times(b, n.table_sb) + pi];
   const int lo = first > base ? first - base : 0;  // tokens [lo, hi) of the block are new, [0, lo) stay
   const int hi = s.kv - base < page ? s.kv - base : page;
 
-  const uint16_t* src = is_v ? (const uint16_t*)p.v + h * p.v_sh : (const uint16_t*)p.k + h * p.k_sh;
+  const uint16_t* src = is_v ? (const uint16_t*)p.v + times(h, p.v_sh) : (const uint16_t*)p.k + times(h, p.k_sh);
   const int64_t sr = is_v ? p.v_sr : p.k_sr;
   float x[TOK][8];
   float amax = 0.f;
@@ -138,7 +136,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   for (int i = 0; i < TOK; ++i) {
     const int t = grp + 16 * i;
     if (t >= lo && t < hi) {
-      load8(src + (int64_t)(s.row0 + base + t - first) * sr + 8 * ln, x[i]);
+      load8(src + times(s.row0 + base + t - first, sr) + 8 * ln, x[i]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
@@ -146,8 +144,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   }
   // (the rows are under way before the page number that they go to is looked at)
   if (id < 0 || id >= c.pages) return;
-  uint8_t* codes = is_v ? (uint8_t*)c.v + id * c.v_sp + h * c.v_sh : (uint8_t*)c.k + id * c.k_sp + h * c.k_sh;
-  uint8_t* scale = is_v ? (uint8_t*)c.v_scale + id * c.vs_sp + h : (uint8_t*)c.k_scale + id * c.ks_sp + h;
+  uint8_t* codes = is_v ? (uint8_t*)c.v + times(id, c.v_sp) + h * c.v_sh : (uint8_t*)c.k + times(id, c.k_sp) + h * c.k_sh;
+  uint8_t* scale = is_v ? (uint8_t*)c.v_scale + times(id, c.vs_sp) + h : (uint8_t*)c.k_scale + times(id, c.ks_sp) + h;
   if (!is_v && p.k_norm_w) {
     float g[8];
     load8((const uint16_t*)p.k_norm_w + 8 * ln, g);
@@ -219,9 +217,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   if (tid == 0) *scale = (uint8_t)(e + 127);
 }
 
-bool rows_ok(const void* p, int64_t sr, int64_t sh) { return ((uintptr_t)p & 15) == 0 && sr % 8 == 0 && sh % 8 == 0; }
+bool below_2_31(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
 
 }  // namespace
+
+bool kv_rows_ok(const void* p, int64_t sr, int64_t sh) {
+  return ((uintptr_t)p & 15) == 0 && sr % 8 == 0 && sh % 8 == 0 && below_2_31(sr) && below_2_31(sh);
+}
 
 int kv_check_cache(const dsx_kv_cache* c, const dsx_kv_batch* n, int64_t total_rows) {
   if (!c || !n) return DSX_ENULL;
@@ -230,6 +232,9 @@ int kv_check_cache(const dsx_kv_cache* c, const dsx_kv_batch* n, int64_t total_r
   if (c->pages < 1 || c->heads < 1 || n->batch < 1 || n->table_pages < 1 || n->table_sb < n->table_pages ||
       n->max_rows < 0 || n->max_rows > (1 << 30) || n->max_kv_len < 0 || n->max_kv_len > (1 << 30) || total_rows < 0 ||
       total_rows > 0x7fffffff || n->max_kv_len > (int64_t)n->table_pages * c->page_size)
+    return DSX_EBADSHAPE;
+  if (!below_2_31(c->k_sp) || !below_2_31(c->v_sp) || !below_2_31(c->ks_sp) || !below_2_31(c->vs_sp) ||
+      !below_2_31(n->table_sb))
     return DSX_EBADSHAPE;
   if (c->k_sp % 16 || c->k_sh % 16 || c->v_sp % 16 || c->v_sh % 16) return DSX_EALIGN;
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return DSX_EALIGN;
@@ -250,8 +255,8 @@ extern "C" int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batc
   if (!p->k || !p->v || (p->q && !p->q_out)) return DSX_ENULL;
   if (p->q && p->heads_q < 1) return DSX_EBADSHAPE;
   if (!(p->norm_eps >= 0.f)) return DSX_EBADSHAPE;
-  if (!rows_ok(p->k, p->k_sr, p->k_sh) || !rows_ok(p->v, p->v_sr, p->v_sh)) return DSX_EALIGN;
-  if (p->q && (!rows_ok(p->q, p->q_sr, p->q_sh) || !rows_ok(p->q_out, p->qo_sr, p->qo_sh))) return DSX_EALIGN;
+  if (!kv_rows_ok(p->k, p->k_sr, p->k_sh) || !kv_rows_ok(p->v, p->v_sr, p->v_sh)) return DSX_EALIGN;
+  if (p->q && (!kv_rows_ok(p->q, p->q_sr, p->q_sh) || !kv_rows_ok(p->q_out, p->qo_sr, p->qo_sh))) return DSX_EALIGN;
   if (((uintptr_t)p->k_norm_w | (uintptr_t)p->q_norm_w | (uintptr_t)p->rope) & 15) return DSX_EALIGN;
   if (p->rope && (p->rope_rows < n.max_kv_len || p->rope_sb % 4 ||
                   (p->rope_sb != 0 && p->rope_sb < p->rope_rows * kKvDim)))
@@ -271,6 +276,13 @@ extern "C" int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batc
   const int64_t total = kv_wgs + (int64_t)n.batch * q_per_seq;
   if (total >= (1ll << 24)) return DSX_EBADSHAPE;  // a launch has fewer than 2^32 threads
   a.q_per_seq = (int)q_per_seq;
+  a.q_per_row = (p->heads_q + kQHeads - 1) / kQHeads;
+  a.by_heads = Divisor::of(c.heads);
+  a.by_blocks = Divisor::of(a.blocks_per_seq);
+  if (q_per_seq > 0) {
+    a.by_q_per_seq = Divisor::of(a.q_per_seq);
+    a.by_q_per_row = Divisor::of(a.q_per_row);
+  }
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)total), block(256);
   switch (c.page_size) {

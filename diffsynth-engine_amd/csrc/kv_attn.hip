@@ -80,7 +80,9 @@ __device__ __forceinline__ int share_of(int total, int n, int x) {  // whose run
   return (int)((((uint64_t)x + 1) * n - 1) / (uint64_t)total);
 }
 
-template <int NQ, bool SHARE>  // 16-row columns of query rows; even shares (a.share) or a.splits pieces of every unit
+// NQ: 16-row columns of query rows.  BLOCKS: (page, head) blocks that a tile may lie in, 2 for pages of 16 tokens.
+// SHARE: even shares (a.share), or a.splits pieces of every unit.
+template <int NQ, int BLOCKS, bool SHARE>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const dsx_kv_cache& c = a.c;
   const int wave = uniform(threadIdx.x >> 6);
@@ -114,7 +116,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const int lane = this_lane(), n16 = lane & 15, g4 = lane >> 4;
   // ---- the next segment: a whole unit or a part of one
   int b, qb = 0, skip = 0, count = 0x3fffffff, piece = -1;  // piece: where a part's result goes
+  int first = wave, stride = kWaves;  // the wave's tiles among the segment's
   KvSeq s;
+  // Without a window the first pages are known before the lengths are, and asked for along with them.
+  const bool early = !SHARE && a.p.window == 0;
+  int pg[BLOCKS] = {};
   if constexpr (SHARE) {
     if (place == head_tiles) {
       place = 0;
@@ -141,7 +147,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     place += count;
     left -= count;
   } else {
-    kv_unit(a, blockIdx.x / (unsigned)a.splits, b, h, qb);
+    const int unit = a.by_splits(blockIdx.x);
+    kv_unit(a, unit, b, h, qb);
+    b = uniform(b);
+    if (a.splits > 1) {
+      first += kWaves * (int)(blockIdx.x - unit * a.splits);
+      stride *= a.splits;
+      piece = blockIdx.x;
+    }
+    if (early) {
+#pragma unroll
+      for (int hf = 0; hf < BLOCKS; ++hf)
+        pg[hf] = a.n.page_table[times(b, a.n.table_sb) +
+                                min(((first + stride * lane) * kTileKeys + 16 * hf) >> a.page_shift, a.n.table_pages - 1)];
+    }
     s = kv_seq(a.n, b, a.p.total_rows);
     left = 0;
   }
@@ -156,21 +175,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   if (again) __syncthreads();  // the LDS of the segment before
 
   // ---- the rows of this block and the keys any of them sees
-  const int row_lo = pr0 / a.group, row_hi = (min(pr0 + 16 * NQ, packed) - 1) / a.group;
+  const int row_lo = a.by_group(pr0), row_hi = a.by_group(min(pr0 + 16 * NQ, packed) - 1);
   int lo_first, hi_first, lo_last, hi_last;
   kv_row_span(s.kv, s.rows, row_lo, a.p.causal, a.p.window, lo_first, hi_first);
   kv_row_span(s.kv, s.rows, row_hi, a.p.causal, a.p.window, lo_last, hi_last);
   const int tile_end = (hi_last + kTileKeys - 1) / kTileKeys;
-  int t_begin = lo_first / kTileKeys;
-  if (!SHARE && a.splits > 1) {
-    count = (max(tile_end - t_begin, 0) + a.splits - 1) / a.splits;
-    skip = (int)(blockIdx.x % (unsigned)a.splits) * count;
-    piece = blockIdx.x;
-  }
-  t_begin += skip;
+  const int t_begin = lo_first / kTileKeys + skip;
   const int t_end = min(t_begin + count, tile_end);
-  // This wave's tiles t_begin + wave + kWaves i, i in [0, tiles); all rows see all keys of those in [in_lo, in_hi).
-  auto tiles_below = [&](int t) { return t > t_begin + wave ? (t - t_begin - wave + kWaves - 1) / kWaves : 0; };
+  // This wave's tiles t_first + stride i, i in [0, tiles); all rows see all keys of those in [in_lo, in_hi).
+  const int t_first = t_begin + first;
+  auto tiles_below = [&](int t) -> int {
+    const unsigned rounds = (unsigned)(t - t_first + stride - 1) / (unsigned)kWaves;
+    return t <= t_first ? 0 : SHARE ? rounds : a.by_splits(rounds);
+  };
   const int tiles = tiles_below(t_end);
   const int in_lo = min(tiles_below((lo_last + kTileKeys - 1) / kTileKeys), tiles);
   const int in_hi = max(min(tiles_below(hi_first / kTileKeys), tiles), in_lo);
@@ -187,32 +204,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const int page_mask = c.page_size - 1;
 
   // Page numbers and scales of 64 of the wave's tiles, one tile per lane: two dependent loads per 64 tiles instead of two
-  // per tile.  scales: k of the halves in bytes 0, 1, v in bytes 2, 3.  Keys behind the last one take its page: what is
-  // loaded for them is not used.
-  int pg[2] = {0, 0}, pg_at = -1;
+  // per tile.  scales: k of the blocks in bytes 0, 1, v in bytes 2, 3.  Keys behind the last one take its page: what is
+  // loaded for them is not used.  (Asked for early, they take the entry that the table has, or its last.)
+  int pg_at = -1;
   uint32_t sc_all = 0;
-  uint32_t ks[2], vs[2];  // scale bytes on their way
-  bool bad[2];
-  auto ask_pages = [&](int chunk) __attribute__((always_inline)) {
+  uint32_t ks[BLOCKS], vs[BLOCKS];  // scale bytes on their way
+  bool bad[BLOCKS];
+  auto ask_pages = [&](int chunk, bool have) __attribute__((always_inline)) {
     const AttnArgs& r = args_again();
     pg_at = chunk;
+    if (!have) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int key = min((t_begin + wave + kWaves * (64 * chunk + lane)) * kTileKeys + 16 * hf, hi_last - 1);
-      pg[hf] = r.n.page_table[b * r.n.table_sb + (key >> r.page_shift)];
+      for (int hf = 0; hf < BLOCKS; ++hf) {
+        const int key = min((t_first + stride * (64 * chunk + lane)) * kTileKeys + 16 * hf, hi_last - 1);
+        pg[hf] = r.n.page_table[times(b, r.n.table_sb) + (key >> r.page_shift)];
+      }
     }
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < BLOCKS; ++hf) {
       bad[hf] = pg[hf] < 0 || pg[hf] >= r.c.pages;
       pg[hf] = bad[hf] ? 0 : pg[hf];
-      ks[hf] = ((const uint8_t*)r.c.k_scale)[pg[hf] * r.c.ks_sp + h];
-      vs[hf] = ((const uint8_t*)r.c.v_scale)[pg[hf] * r.c.vs_sp + h];
+      ks[hf] = ((const uint8_t*)r.c.k_scale)[times(pg[hf], r.c.ks_sp) + h];
+      vs[hf] = ((const uint8_t*)r.c.v_scale)[times(pg[hf], r.c.vs_sp) + h];
     }
   };
   auto take_scales = [&]() __attribute__((always_inline)) {
     sc_all = 0;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < BLOCKS; ++hf) {
       // (no scale: NaN scores for every row that sees the block, and nothing for the others)
       const bool none = bad[hf] || vs[hf] == 255;
       sc_all |= ((none ? 255u : ks[hf]) << (8 * hf)) | ((none ? 127u : vs[hf]) << (16 + 8 * hf));
@@ -220,24 +239,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   };
   auto scales_at = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)sc_all, i & 63); };
   auto load_codes = [&](int i, TileRegs& r) __attribute__((always_inline)) {
-    const int key = (t_begin + wave + kWaves * i) * kTileKeys;
+    const int key = (t_first + stride * i) * kTileKeys;
     uint32_t ko = koff, vo = voff;
     asm volatile("" : "+v"(ko), "+v"(vo));  // (32-bit offsets to a scalar base; widened outside, they would be 64-bit sums)
+    const uint8_t *kp, *vp;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int64_t page = __builtin_amdgcn_readlane(pg[hf], i & 63);
-      const int tok = (key + 16 * hf) & page_mask;
-      const uint8_t* kp = kbase + page * c.k_sp + tok * kKvDim;
-      const uint8_t* vp = vbase + page * c.v_sp + tok * kKvDim;
+      if (hf < BLOCKS) {
+        const int page = __builtin_amdgcn_readlane(pg[hf], i & 63);
+        const int tok = (key + 16 * hf) & page_mask;
+        kp = kbase + times(page, c.k_sp) + tok * kKvDim;
+        vp = vbase + times(page, c.v_sp) + tok * kKvDim;
+      }
+      const int more = hf < BLOCKS ? 0 : 16 * kKvDim;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) r.k[hf][w] = *reinterpret_cast<const u32x4*>(kp + ko + 64 * w);
+      for (int w = 0; w < 2; ++w) r.k[hf][w] = *reinterpret_cast<const u32x4*>(kp + ko + 64 * w + more);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) r.v[hf][t] = *reinterpret_cast<const u32x2*>(vp + vo + t * kKvDim);
+      for (int t = 0; t < 4; ++t) r.v[hf][t] = *reinterpret_cast<const u32x2*>(vp + vo + t * kKvDim + more);
     }
   };
   auto load_tile = [&](int i, TileRegs& r) __attribute__((always_inline)) -> uint32_t {  // returns its scales
     if ((i >> 6) != pg_at) {
-      ask_pages(i >> 6);
+      ask_pages(i >> 6, false);
       take_scales();
     }
     load_codes(i, r);
@@ -254,7 +277,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
   const bool near = (in_lo + kRing - 2) >> 6 == chunk;
   if (tiles > 0) {
     // (the first codes are asked for along with the scales, not behind them)
-    ask_pages(chunk);
+    ask_pages(chunk, early && chunk == 0);
     if (first_masked < tiles) load_codes(first_masked, ring[kRing - 1]);
 #pragma unroll
     for (int r = 0; r < kRing - 1; ++r)
@@ -286,7 +309,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 
   auto compute = [&](auto masked, int i, TileRegs& r, uint32_t sc) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
-    const int key0 = (t_begin + wave + kWaves * i) * kTileKeys;
+    const int key0 = (t_first + stride * i) * kTileKeys;
     f32x4 st[2][NQ];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -295,11 +318,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
       const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
-        st[hf][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].lo, z, 0, 0, 0, (int)(sc >> (8 * hf)), 0, qf[q].s_lo);
+        st[hf][q] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].lo, z, 0, 0, 0, (int)(sc >> (8 * (hf % BLOCKS))), 0, qf[q].s_lo);
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
         st[hf][q] =
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].hi, st[hf][q], 0, 0, 0, (int)(sc >> (8 * hf)), 0, qf[q].s_hi);
+            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[q].hi, st[hf][q], 0, 0, 0, (int)(sc >> (8 * (hf % BLOCKS))), 0, qf[q].s_hi);
     }
     bool has_nan = false;
     if constexpr (kMasked) {
@@ -331,9 +354,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const f32x4& v = st[hf][q];
-        mx[hf] = __builtin_fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), cs, ev[hf]);
+        mx[hf] = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
       }
-      const float top = quad_max(fmaxf(mx[0], mx[1]));
+      const float top = quad_max(BLOCKS == 1 ? __builtin_fmaf(fmaxf(mx[0], mx[1]), cs, ev[0])
+                                             : fmaxf(__builtin_fmaf(mx[0], cs, ev[0]), __builtin_fmaf(mx[1], cs, ev[1])));
       if (__builtin_amdgcn_ballot_w64(top > m_run[q]) != 0) {
         const float m_new = fmaxf(m_run[q], top);
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[q] - m_new);
@@ -346,16 +370,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
       }
       const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
       u32x4 pw;
+      float sum = 0.f;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const float off = ev[hf] + kHeadroom - ref;
-        float w[4], sum = 0.f;
+        const float off = ev[hf % BLOCKS] + kHeadroom - ref;
+        float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[hf][q][e], cs, off));
           sum += w[e];
         }
-        l_run[q] = __builtin_fmaf(sum, inv_v[hf], l_run[q]);
+        if (BLOCKS == 2 || hf == 1) {
+          l_run[q] = __builtin_fmaf(sum, inv_v[hf % BLOCKS], l_run[q]);
+          sum = 0.f;
+        }
         pw[2 * hf] = pack_f16x2(w[0], w[1]);
         pw[2 * hf + 1] = pack_f16x2(w[2], w[3]);
       }
@@ -487,8 +515,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
       } else {
         const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
         const u32x2 w = {pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
-        const int row = pr / a.group, hh = h * a.group + pr % a.group;
-        *reinterpret_cast<u32x2*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+        const int row = a.by_group(pr), hh = h * a.group + pr - row * a.group;
+        *reinterpret_cast<u32x2*>((uint16_t*)a.p.out + times(s.row0 + row, a.p.o_sr) + times(hh, a.p.o_sh) + d0) = w;
       }
     }
   }
@@ -498,15 +526,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
 // Joins the pieces of split key ranges.  16 lanes x 8 elements read one piece of one packed query row; the 16 such groups
 // of a workgroup take `ways` pieces of 16 / ways rows at once (ways: the number of pieces, up to a power of two and 16)
 // and meet in LDS in a fixed order.  All pieces behind one another in a lane took 25 us for 26 of them.
-__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
+__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways_log2, Divisor by_blocks) {
   const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
   __shared__ float sm_o[16][kKvDim + 4];
   __shared__ float sm_m[16], sm_l[16];
   asm volatile("" ::"s"(a.n.row_start), "s"(a.p.out), "s"(a.p.total_rows), "s"(a.part_o));
-  const int per = 16 / ways, slot = grp / ways, way = grp % ways;
-  const int blocks = (a.block_rows + per - 1) / per;
-  const int64_t cut = blockIdx.x / (unsigned)blocks;  // the unit, counted from the first that is cut
-  const int r = (int)(blockIdx.x % (unsigned)blocks) * per + slot;
+  const int ways = 1 << ways_log2, per = 16 >> ways_log2, slot = grp >> ways_log2, way = grp & (ways - 1);
+  const int blocks = (a.block_rows + per - 1) >> (4 - ways_log2);
+  const int64_t cut = by_blocks(blockIdx.x);  // the unit, counted from the first that is cut
+  const int r = (int)(blockIdx.x - cut * blocks) * per + slot;
   int b, h, qb;
   kv_unit(a, (uint32_t)(a.first_split + cut), b, h, qb);
   const KvSeq s = kv_seq(a.n, b, a.p.total_rows);
@@ -578,13 +606,13 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a, int ways) {
   u32x4 w;
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  const int row = pr / a.group, hh = h * a.group + pr % a.group;
-  *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + d0) = w;
+  const int row = a.by_group(pr), hh = h * a.group + pr - row * a.group;
+  *reinterpret_cast<u32x4*>((uint16_t*)a.p.out + times(s.row0 + row, a.p.o_sr) + times(hh, a.p.o_sh) + d0) = w;
 }
 
 struct Plan {
   int nq;  // 16-row columns of the streaming form; 0: the tile form
-  int block_rows, nqb, share, splits, ways;
+  int block_rows, nqb, share, splits, ways, ways_log2;
   int64_t units, first_split, join_units, ws_bytes;
 };
 
@@ -647,28 +675,30 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
     r.join_units = tail;
     r.ways = r.splits;
   }
-  int ways = 1;
-  while (ways < r.ways && ways < 16) ways *= 2;
-  r.ways = ways;
+  while ((1 << r.ways_log2) < r.ways && r.ways_log2 < 4) ++r.ways_log2;
   r.ws_bytes = pieces * r.block_rows * (kKvDim + 2) * 4;
   return r;
 }
 
-template <int NQ, bool SHARE>
+template <int NQ, int BLOCKS, bool SHARE>
 int launch_stream(const AttnArgs& a, unsigned workgroups, hipStream_t st) {
   static PerDeviceOnce attr_once;
   const int rc = per_device_once(attr_once, [](int) {
-    return hipFuncSetAttribute((const void*)kv_stream_kernel<NQ, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize,
+    return hipFuncSetAttribute((const void*)kv_stream_kernel<NQ, BLOCKS, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                (int)sizeof(StreamLds)) == hipSuccess ? (int)DSX_OK : (int)DSX_ELAUNCH;
   });
   if (rc != DSX_OK) return rc;
-  kv_stream_kernel<NQ, SHARE><<<dim3(workgroups), dim3(64 * kWaves), sizeof(StreamLds), st>>>(a);
+  kv_stream_kernel<NQ, BLOCKS, SHARE><<<dim3(workgroups), dim3(64 * kWaves), sizeof(StreamLds), st>>>(a);
   return DSX_OK;
+}
+template <int NQ, int BLOCKS>
+int launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
+  return a.share ? launch_stream<NQ, BLOCKS, true>(a, (unsigned)a.share, st)
+                 : launch_stream<NQ, BLOCKS, false>(a, (unsigned)(units * a.splits), st);
 }
 template <int NQ>
 int launch_stream(const AttnArgs& a, int64_t units, hipStream_t st) {
-  return a.share ? launch_stream<NQ, true>(a, (unsigned)a.share, st)
-                 : launch_stream<NQ, false>(a, (unsigned)(units * a.splits), st);
+  return a.c.page_size >= kTileKeys ? launch_stream<NQ, 1>(a, units, st) : launch_stream<NQ, 2>(a, units, st);
 }
 
 }  // namespace
@@ -689,8 +719,7 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
   const dsx_kv_cache& c = *cache;
   const dsx_kv_batch& n = *batch;
   if (!p->q || !p->out) return DSX_ENULL;
-  if ((((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->workspace) & 15) || p->q_sr % 8 || p->q_sh % 8 ||
-      p->o_sr % 8 || p->o_sh % 8)
+  if (!kv_rows_ok(p->q, p->q_sr, p->q_sh) || !kv_rows_ok(p->out, p->o_sr, p->o_sh) || ((uintptr_t)p->workspace & 15))
     return DSX_EALIGN;
   if (n.max_rows == 0 || p->total_rows == 0) return DSX_OK;
   Plan plan = make_plan(c, n, *p);
@@ -704,8 +733,8 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
       return DSX_EWORKSPACE;
     }
   }
-  const int per = 16 / plan.ways;
-  const int64_t join_wgs = plan.join_units * ((plan.block_rows + per - 1) / per);
+  const int per = 16 >> plan.ways_log2, join_blocks = (plan.block_rows + per - 1) / per;
+  const int64_t join_wgs = plan.join_units * join_blocks;
   // A launch has fewer than 2^32 threads: 512 a unit (and a few more where the tile form cuts some), 256 a join.
   if (plan.units >= (1ll << 23) - 4096 || join_wgs >= (1ll << 24)) return DSX_EBADSHAPE;
   AttnArgs a{};
@@ -719,6 +748,10 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
   a.share = plan.share;
   a.splits = plan.splits;
   a.first_split = plan.first_split;
+  a.by_group = Divisor::of(a.group);
+  a.by_nqb = Divisor::of(a.nqb);
+  a.by_batch = Divisor::of(n.batch);
+  a.by_splits = Divisor::of(a.splits);
   if (plan.join_units > 0) {
     a.part_o = (float*)p->workspace;
     a.part_ml = a.part_o + plan.ws_bytes / (4 * (kKvDim + 2)) * kKvDim;
@@ -729,6 +762,7 @@ extern "C" int dsx_kv_attn(const dsx_kv_cache* cache, const dsx_kv_batch* batch,
                                  : launch_kv_tile(a, plan.units, st);
   if (lrc != DSX_OK) return lrc;
   if (hipGetLastError() != hipSuccess) return DSX_ELAUNCH;
-  if (join_wgs > 0) kv_join_kernel<<<dim3((unsigned)join_wgs), dim3(256), 0, st>>>(a, plan.ways);
+  if (join_wgs > 0)
+    kv_join_kernel<<<dim3((unsigned)join_wgs), dim3(256), 0, st>>>(a, plan.ways_log2, Divisor::of(join_blocks));
   return hipGetLastError() == hipSuccess ? DSX_OK : DSX_ELAUNCH;
 }

@@ -22,16 +22,17 @@ struct AttnArgs {
   int splits;           // into so many pieces of their key ranges
   float* part_o;   // (pieces, block_rows, 128) fp32
   float* part_ml;  // (pieces, block_rows, 2)
+  Divisor by_group, by_nqb, by_batch, by_splits;
 };
 
 // Unit number -> (sequence, cache head, query block).  Sequences inside heads: runs of units (the tile form gives each XCD
 // one) then hold all sequences alike, long and short.  Causal blocks come last first: they are the longest.
 __device__ __forceinline__ void kv_unit(const AttnArgs& a, uint32_t unit, int& b, int& h, int& qb) {
-  qb = (int)(unit % (uint32_t)a.nqb);
+  const uint32_t blocks = a.by_nqb(unit);
+  qb = (int)(unit - blocks * a.nqb);
   if (a.p.causal) qb = a.nqb - 1 - qb;
-  unit /= (uint32_t)a.nqb;
-  b = (int)(unit % (uint32_t)a.n.batch);
-  h = (int)(unit / (uint32_t)a.n.batch);
+  h = (int)a.by_batch(blocks);
+  b = (int)(blocks - (uint32_t)h * a.n.batch);
 }
 
 // Inclusive sum over the lanes of a wave: six adds, each fed by the row shifts and broadcasts of the vector unit.
@@ -86,9 +87,9 @@ struct QRaw {
 };
 __device__ __forceinline__ void load_q(const AttnArgs& a, const KvSeq& s, int h, int pr, int g4, QRaw& raw, int& lo,
                                        int& hi) {
-  const int row = pr / a.group, hh = h * a.group + pr % a.group;
+  const int row = a.by_group(pr), hh = h * a.group + pr - row * a.group;
   kv_row_span(s.kv, s.rows, row, a.p.causal, a.p.window, lo, hi);
-  const uint16_t* src = (const uint16_t*)a.p.q + (int64_t)(s.row0 + row) * a.p.q_sr + hh * a.p.q_sh + 16 * g4;
+  const uint16_t* src = (const uint16_t*)a.p.q + times(s.row0 + row, a.p.q_sr) + times(hh, a.p.q_sh) + 16 * g4;
 #pragma unroll
   for (int w = 0; w < 4; ++w) raw.w[w] = *reinterpret_cast<const u32x4*>(src + 64 * (w >> 1) + 8 * (w & 1));
 }

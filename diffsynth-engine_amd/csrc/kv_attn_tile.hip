@@ -68,8 +68,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     const unsigned j = blockIdx.x - whole8;
     const unsigned piece = (j & 7) * (unsigned)(cut8 >> 3) + (j >> 3);
     if (piece >= (units - a.first_split) * a.splits) return;
-    unit = a.first_split + piece / (unsigned)a.splits;
-    split = (int)(piece % (unsigned)a.splits);
+    const unsigned cut = a.by_splits(piece);
+    unit = a.first_split + cut;
+    split = (int)(piece - cut * a.splits);
     splits = a.splits;
   }
   int b, h, qb;
@@ -87,12 +88,12 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
   // ---- spans: of the workgroup (first and last row), of the wave, of the lane's two rows
   const int causal = a.p.causal, window = a.p.window;
   int lo_first, hi_first, lo_last, hi_last, wlo_first, whi_first, wlo_last, whi_last;
-  kv_row_span(s.kv, s.rows, pr0 / a.group, causal, window, lo_first, hi_first);
-  kv_row_span(s.kv, s.rows, (min(pr0 + kTileRows, packed) - 1) / a.group, causal, window, lo_last, hi_last);
+  kv_row_span(s.kv, s.rows, a.by_group(pr0), causal, window, lo_first, hi_first);
+  kv_row_span(s.kv, s.rows, a.by_group(min(pr0 + kTileRows, packed) - 1), causal, window, lo_last, hi_last);
   const int wr0 = pr0 + wave * 32;
   const bool active = wr0 < packed;
-  kv_row_span(s.kv, s.rows, min(wr0, packed - 1) / a.group, causal, window, wlo_first, whi_first);
-  kv_row_span(s.kv, s.rows, min(wr0 + 31, packed - 1) / a.group, causal, window, wlo_last, whi_last);
+  kv_row_span(s.kv, s.rows, a.by_group(min(wr0, packed - 1)), causal, window, wlo_first, whi_first);
+  kv_row_span(s.kv, s.rows, a.by_group(min(wr0 + 31, packed - 1)), causal, window, wlo_last, whi_last);
   const int tile_first = lo_first / KB, tile_last = (hi_last + KB - 1) / KB;
   const int per = (max(tile_last - tile_first, 0) + splits - 1) / splits;
   const int kb_begin = tile_first + split * per;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       if (__builtin_expect(i - pg_at >= 64, 0)) {
         const AttnArgs& r = args_again();
         pg_at = i & ~63;
-        const int id = r.n.page_table[b * r.n.table_sb +
+        const int id = r.n.page_table[times(b, r.n.table_sb) +
                                       (min((kb_begin + pg_at + lane) * KB + 8 * wave, hi_last - 1) >> r.page_shift)];
         pg = id < 0 || id >= r.c.pages ? 0 : id;
       }
@@ -147,12 +148,12 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
         ks_all = vs_all = 0;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-          const int id = r.n.page_table[b * r.n.table_sb +
+          const int id = r.n.page_table[times(b, r.n.table_sb) +
                                         (min((kb_begin + sc_at + lane) * KB + 16 * q, hi_last - 1) >> r.page_shift)];
           const bool bad = id < 0 || id >= r.c.pages;
-          const int64_t page = bad ? 0 : id;
-          uint32_t k8 = ((const uint8_t*)r.c.k_scale)[page * r.c.ks_sp + h];
-          uint32_t v8 = ((const uint8_t*)r.c.v_scale)[page * r.c.vs_sp + h];
+          const int page = bad ? 0 : id;
+          uint32_t k8 = ((const uint8_t*)r.c.k_scale)[times(page, r.c.ks_sp) + h];
+          uint32_t v8 = ((const uint8_t*)r.c.v_scale)[times(page, r.c.vs_sp) + h];
           if (bad || v8 == 255) {  // NaN scores for every row that sees the block, and nothing for the others
             k8 = 255;
             v8 = 127;
@@ -187,10 +188,10 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       src = (int64_t)((kb * KB + 8 * wave) & page_mask) * kKvDim;
     };
     auto issue_k = [&](int stage) {
-      dma16(kbase + src_page * c.k_sp + src, off_k, lds0 + stage * kRaw + wave * 1024);
+      dma16(kbase + times(src_page, c.k_sp) + src, off_k, lds0 + stage * kRaw + wave * 1024);
     };
     auto issue_v = [&](int stage) {
-      dma16(vbase + src_page * c.v_sp + src, off_v, lds0 + kOffV + stage * kRaw + wave * 1024);
+      dma16(vbase + times(src_page, c.v_sp) + src, off_v, lds0 + kOffV + stage * kRaw + wave * 1024);
     };
 
     // Some row of the workgroup does not see some key of the tile.
@@ -616,8 +617,8 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       }
     } else if (pr < packed) {
       const float inv = s.ok ? (l == 0.f ? 0.f : 1.f / l) : NAN;
-      const int row = pr / a.group, hh = h * a.group + pr % a.group;
-      uint16_t* dst = (uint16_t*)a.p.out + (int64_t)(s.row0 + row) * a.p.o_sr + hh * a.p.o_sh + 32 * g4;
+      const int row = a.by_group(pr), hh = h * a.group + pr - row * a.group;
+      uint16_t* dst = (uint16_t*)a.p.out + times(s.row0 + row, a.p.o_sr) + times(hh, a.p.o_sh) + 32 * g4;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         u32x4 w;

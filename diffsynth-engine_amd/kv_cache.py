@@ -52,6 +52,8 @@ class KVCache(_Fixed):
                 raise ValueError("KVCache: codes must be float8_e4m3fn, got %s" % t.dtype)
             if t.stride(3) != 1 or t.stride(2) != HEAD_DIM or t.stride(1) % 16 or t.stride(0) % 16 or t.data_ptr() % 16:
                 raise ValueError("KVCache: every (page, head) block must be contiguous and 16-byte aligned")
+            if t.stride(0) > 0x7fffffff:
+                raise ValueError("KVCache: page strides must be below 2^31")
             if not _apart(t.shape[:2], t.stride()[:2], t.shape[2] * HEAD_DIM):
                 raise ValueError("KVCache: blocks overlap in memory")
         for t in (k_scale, v_scale):

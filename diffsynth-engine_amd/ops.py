@@ -650,9 +650,9 @@ def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None)
                          % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(shape)))
     sr, sh, sd = t.stride()
     ptr = t.data_ptr()
-    if sd != 1 or sr % 8 or sh % 8 or ptr % 16:
-        raise ValueError("%s needs unit stride in the head dim, other strides in multiples of 8 and 16-byte alignment"
-                         % name)
+    if sd != 1 or sr % 8 or sh % 8 or ptr % 16 or sr > 0x7fffffff or sh > 0x7fffffff:
+        raise ValueError("%s needs unit stride in the head dim, other strides in multiples of 8 (below 2^31) and 16-byte "
+                         "alignment" % name)
     return ptr, sr, sh
 
 

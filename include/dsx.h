@@ -391,6 +391,7 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
  * whose lengths break one is not appended and its rows (as far as they lie in the output) leave attention as NaN; a
  * page number outside [0, pages) is not written, and rows that see a token of it become NaN.  dsx_kv_plan_check does the
  * same checks on the host.
+ * Row and head strides of q, k, v and the outputs lie in [0, 2^31) elements.
  * Rows from row_start[batch] on belong to nobody and are left as they are.
  * The bounds also limit a launch (DSX_EBADSHAPE beyond): attention to 2^23 - 4096 units of (sequence, cache head, block of
  * 16, 32 or 256 query rows), an append to 2^24 blocks of (sequence, page that max_rows rows can reach, head).
@@ -398,8 +399,8 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
 typedef struct dsx_kv_cache {
   void* k; void* v;
   void* k_scale; void* v_scale;
-  int64_t k_sp, k_sh, v_sp, v_sh;    /* page and head strides of the codes, multiples of 16 */
-  int64_t ks_sp, vs_sp;              /* page strides of the scales */
+  int64_t k_sp, k_sh, v_sp, v_sh;    /* page and head strides of the codes, multiples of 16; page strides < 2^31 */
+  int64_t ks_sp, vs_sp;              /* page strides of the scales, < 2^31 */
   int32_t pages, heads, page_size;   /* page_size: 16, 32, 64 or 128 tokens */
 } dsx_kv_cache;
 
@@ -407,7 +408,7 @@ typedef struct dsx_kv_batch {
   const int32_t* page_table; int64_t table_sb;
   const int32_t* row_start;
   const int32_t* kv_len;
-  int32_t batch, table_pages;        /* table_pages: columns of page_table, table_sb >= table_pages */
+  int32_t batch, table_pages;        /* table_pages: columns of page_table, table_pages <= table_sb < 2^31 */
   int32_t max_rows, max_kv_len;      /* max_kv_len <= table_pages * page_size; both <= 2^30 */
 } dsx_kv_batch;
 

@@ -171,6 +171,9 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
             assert call(n=changed(plan._c, **kw)) == _lib.DSX_ENULL
         for kw in (dict(page_size=24), dict(pages=0), dict(heads=0)):
             assert call(c=changed(cache._c, **kw)) == _lib.DSX_EBADSHAPE
+        for kw in (dict(k_sp=2 ** 31), dict(v_sp=-2048), dict(ks_sp=2 ** 31), dict(vs_sp=-2)):
+            assert call(c=changed(cache._c, **kw)) == _lib.DSX_EBADSHAPE
+        assert call(n=changed(plan._c, table_sb=2 ** 31)) == _lib.DSX_EBADSHAPE
         for kw in (dict(k_sp=2056), dict(v_sh=8), dict(k=at + 8)):
             assert call(c=changed(cache._c, **kw)) == _lib.DSX_EALIGN
         for kw in (dict(batch=0), dict(table_pages=0), dict(table_sb=1), dict(max_rows=-1), dict(max_kv_len=33),
@@ -180,7 +183,7 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
         assert call(total_rows=2 ** 31) == _lib.DSX_EBADSHAPE
         assert call(total_rows=0) == _lib.DSX_OK  # nothing to do, nothing launched
     for kw, rc in ((dict(q=None), _lib.DSX_ENULL), (dict(out=None), _lib.DSX_ENULL), (dict(q=at + 2), _lib.DSX_EALIGN),
-                   (dict(o_sr=252), _lib.DSX_EALIGN), (dict(heads_q=3), _lib.DSX_EBADSHAPE),
+                   (dict(o_sr=252), _lib.DSX_EALIGN), (dict(q_sr=2 ** 31), _lib.DSX_EALIGN), (dict(o_sh=-128), _lib.DSX_EALIGN), (dict(heads_q=3), _lib.DSX_EBADSHAPE),
                    (dict(heads_q=0), _lib.DSX_EBADSHAPE), (dict(window=-1), _lib.DSX_EBADSHAPE),
                    (dict(softmax_scale=0.0), _lib.DSX_EBADSHAPE), (dict(softmax_scale=math.nan), _lib.DSX_EBADSHAPE),
                    (dict(softmax_scale=math.inf), _lib.DSX_EBADSHAPE), (dict(softmax_scale=-1.0), _lib.DSX_EBADSHAPE),
@@ -193,7 +196,7 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
     assert attn(n=long, workspace=at, workspace_bytes=need - 1) == _lib.DSX_EWORKSPACE
     for kw, rc in ((dict(k=None), _lib.DSX_ENULL), (dict(v=None), _lib.DSX_ENULL), (dict(q=at), _lib.DSX_ENULL),
                    (dict(q=at, q_out=at), _lib.DSX_EBADSHAPE), (dict(k=at + 2), _lib.DSX_EALIGN),
-                   (dict(v_sr=100), _lib.DSX_EALIGN), (dict(q=at, q_out=at + 2, heads_q=1), _lib.DSX_EALIGN),
+                   (dict(v_sr=100), _lib.DSX_EALIGN), (dict(k_sh=-128), _lib.DSX_EALIGN), (dict(q=at, q_out=at + 2, heads_q=1), _lib.DSX_EALIGN),
                    (dict(k_norm_w=at + 2), _lib.DSX_EALIGN), (dict(norm_eps=-1.0), _lib.DSX_EBADSHAPE),
                    (dict(norm_eps=math.nan), _lib.DSX_EBADSHAPE), (dict(rope=at, rope_rows=31), _lib.DSX_EBADSHAPE),
                    (dict(rope=at, rope_rows=32, rope_sb=128), _lib.DSX_EBADSHAPE)):
