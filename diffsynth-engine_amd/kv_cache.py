@@ -140,8 +140,8 @@ class KVPlan(_Fixed):
             raise ValueError("KVPlan: sequence %d (rows [%d, %d), %d tokens) breaks a bound"
                              % (b, starts[b], starts[b + 1], lens[b]) if b >= 0 else _lib.strerror(rc))
 
-    def _fits(self, cache: KVCache, index: Optional[int] = None):
-        if cache._index != self._index or (index is not None and index != self._index):
+    def _fits(self, cache: KVCache):
+        if cache._index != self._index:
             raise ValueError("the rows, the cache and the plan must be on one device")
         if self.max_kv_len > self.table_pages * cache.page_size:
             raise ValueError("KVPlan: %d pages of %d tokens cannot hold max_kv_len = %d"

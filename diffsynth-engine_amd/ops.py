@@ -643,14 +643,17 @@ def flow_match_euler_step(latents: torch.Tensor, model_outputs: torch.Tensor, dt
 
 def _kv_rows(name: str, t: torch.Tensor, rows: int, heads: Optional[int] = None):
     """(pointer, row stride, head stride) of a (rows, heads, 128) bf16 view."""
-    shape = t.shape
-    if t.dtype != _BF16 or len(shape) != 3 or shape[0] != rows or shape[2] != HEAD_DIM \
-            or (heads is not None and shape[1] != heads):
+    if t.dtype != _BF16 or t.dim() != 3:
+        r = h = d = -1
+    else:
+        r, h, d = t.shape
+    if r != rows or d != HEAD_DIM or (h != heads and heads is not None):
         raise ValueError("%s must be bf16 (%d, %s, 128), got %s %s"
-                         % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(shape)))
+                         % (name, rows, "heads" if heads is None else heads, t.dtype, tuple(t.shape)))
     sr, sh, sd = t.stride()
     ptr = t.data_ptr()
-    if sd != 1 or sr % 8 or sh % 8 or ptr % 16 or sr > 0x7fffffff or sh > 0x7fffffff:
+    both = sr | sh
+    if sd != 1 or both & 7 or ptr & 15 or both > 0x7fffffff:
         raise ValueError("%s needs unit stride in the head dim, other strides in multiples of 8 (below 2^31) and 16-byte "
                          "alignment" % name)
     return ptr, sr, sh
@@ -665,34 +668,34 @@ def _kv_apart(name: str, rows: int, heads: int, sr: int, sh: int):
 
 def _kv_device(name: str, cache: KVCache, plan: KVPlan, *tensors) -> int:
     """The one device that everything is on (a number: these calls are short, and device objects take a while)."""
-    index = tensors[0].get_device()
+    index = plan._index
     for t in tensors:
         if t is not None and t.get_device() != index:
             _require_cuda(*tensors)
-            raise ValueError("%s: all tensors must be on one device" % name)
+            raise ValueError("%s: the rows, the cache and the plan must be on one device" % name)
     if index < 0:
         _require_cuda(*tensors)
-    plan._fits(cache, index)
+    plan._fits(cache)
     return index
 
 
 def _kv_call(fn, what: str, index: int, *args):
     """Calls the library with the tensors' device current and that device's current stream."""
-    if index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
-def _kv_norm_weight(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if w is None:
-        return None
+def _kv_norm_weight(w: torch.Tensor) -> torch.Tensor:
     if w.numel() != HEAD_DIM:
         raise ValueError("kv_append: RMSNorm weights have 128 entries")
     if w.dtype != _BF16 or not w.is_contiguous():
         w = w.to(_BF16).contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+    return w if w.data_ptr() & 15 == 0 else w.clone()
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
@@ -730,17 +733,24 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
         qp, q_sr, q_sh = _kv_rows("kv_append: q", q, rows)
         heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
-        qop, qo_sr, qo_sh = _kv_rows("kv_append: q_out", q_out, rows, heads)
-        _kv_apart("kv_append: q_out", rows, heads, qo_sr, qo_sh)
-    k_norm_w, q_norm_w = _kv_norm_weight(k_norm_w), _kv_norm_weight(q_norm_w)
+            q_out = q.new_empty((rows, heads, HEAD_DIM))
+            qop, qo_sr, qo_sh = q_out.data_ptr(), heads * HEAD_DIM, HEAD_DIM
+        else:
+            qop, qo_sr, qo_sh = _kv_rows("kv_append: q_out", q_out, rows, heads)
+            _kv_apart("kv_append: q_out", rows, heads, qo_sr, qo_sh)
+    if k_norm_w is not None:
+        k_norm_w = _kv_norm_weight(k_norm_w)
+    if q_norm_w is not None:
+        q_norm_w = _kv_norm_weight(q_norm_w)
     rope_sb = rope_rows = 0
     if rope is not None:
         rope = _rope_table(rope, plan.batch, plan.max_kv_len)
         rope_rows = rope.shape[1]
         rope_sb = rope.stride(0) if rope.shape[0] > 1 else 0
-    if not rows or (q is not None and not heads):
+    if not rows:
         return q_out
+    if not heads:
+        qp = None  # (a q without heads: nothing of it to prepare)
     p = _lib.KVAppendParams(kp, k_sr, k_sh, vp, v_sr, v_sh, qp, q_sr, q_sh, qop, qo_sr, qo_sh, _ptr(k_norm_w),
                             _ptr(q_norm_w), _ptr(rope), rope_sb, rope_rows, rows, eps, heads)
     _kv_call(_lib.load().dsx_kv_append, "dsx_kv_append", index, cache._ref, plan._ref, ctypes.byref(p))
@@ -774,9 +784,11 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     if not 0.0 < scale < 3e38:
         raise ValueError("kv_attention: scale must be positive and finite")
     if out is None:
-        out = torch.empty((rows, heads, HEAD_DIM), dtype=_BF16, device=q.device)
-    op, o_sr, o_sh = _kv_rows("kv_attention: out", out, rows, heads)
-    _kv_apart("kv_attention: out", rows, heads, o_sr, o_sh)
+        out = q.new_empty((rows, heads, HEAD_DIM))
+        op, o_sr, o_sh = out.data_ptr(), heads * HEAD_DIM, HEAD_DIM
+    else:
+        op, o_sr, o_sh = _kv_rows("kv_attention: out", out, rows, heads)
+        _kv_apart("kv_attention: out", rows, heads, o_sr, o_sh)
     if not rows:
         return out
     lib = _lib.load()
@@ -784,7 +796,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     ref = ctypes.byref(p)
     need = lib.dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, ref) if split_keys else 0
     if need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need // 2)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
     _kv_call(lib.dsx_kv_attn, "dsx_kv_attn", index, cache._ref, plan._ref, ref)
     return out

@@ -728,3 +728,16 @@ def test_outputs_that_overlap_are_refused(dev):
             ops.kv_append(k, v, c.cache, c.plan, q=q, q_out=bad)
     out = flat.view(5, 9, 128)[:, 1:8:2]  # every other head of a wider buffer
     assert torch.equal(ops.kv_attention(q, c.cache, c.plan, out=out), ops.kv_attention(q, c.cache, c.plan))
+
+
+def test_a_q_without_heads_does_not_keep_k_and_v_out(dev):
+    from diffsynth_engine_amd import ops
+
+    c, d = (Case(dev, [3, 1], [20, 40], page=16, seed=7) for _ in range(2))
+    q = torch.empty(4, 0, 128, dtype=BF, device=dev)
+    assert ops.kv_append(c.k.to(dev), c.v.to(dev), c.cache, c.plan, q=q).shape == q.shape
+    ops.kv_append(d.k.to(dev), d.v.to(dev), d.cache, d.plan)
+    a, b = c.pull(), d.pull()
+    assert all(torch.equal(a[n].view(torch.uint8), b[n].view(torch.uint8)) and torch.equal(a[n + "_scale"], b[n + "_scale"])
+               for n in "kv")
+    assert not torch.equal(a["k"].view(torch.uint8), c.host["k"].view(torch.uint8))
