@@ -648,18 +648,20 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   int64_t pieces = 0;
   if (r.nq) {
     const int64_t tiles = (span + kTileKeys - 1) / kTileKeys + 1;
-    // The longest a compute unit's share can be, in tiles.  From 512 on, even shares and a join (which costs 6 us) beat one
-    // workgroup per unit and its uneven end: 64 x 16384 tokens, 8 heads (1024 tiles): 288 against 305 us; 32 x 16384 (512):
-    // 173 against 178; 32 x 8192 (256): 93 against 90; 32 x 4097 (129): 58 against 46.  Fewer units than compute units are
-    // cut into equal pieces of at least a tile a wave (pieces of two or four tiles bring nothing: 1561 tokens, 12 heads,
-    // 13.3 against 13.6 and 14.5 us).
+    // The longest a compute unit's share can be, in tiles.  From 512 on, even shares and a join (which costs 5 us) beat one
+    // workgroup per unit and its uneven end: 64 x 16384 tokens, 8 heads (1024 tiles): 280 against 305 us; 32 x 16384 (512):
+    // 168 against 178; 32 x 8192 (256): 93 against 86; 32 x 4097 (129): 58 against 44.
+    // Fewer units than compute units are cut into equal pieces, as many as there are compute units and tiles for the waves,
+    // from four tiles a wave on: 1 x 1561 tokens, 12 heads (six pieces): 11.6 against 14.5 us, 1000 tokens: 10.6 against
+    // 12.1; below that the join costs more than it saves: 4 x 5 rows, 4 heads, 800 tokens: 15.4 against 14.9, 500: 14.0
+    // against 12.6.  Fewer, longer pieces bring nothing (1561 tokens in three: 12.7).
     const int64_t load = r.units * tiles / cus;
     if (load >= 512 && r.nqb == 1 && r.units * tiles < (1ll << 30)) {
       r.share = cus;
       pieces = 2 * (int64_t)r.share;
       r.ways = (int)((r.share + r.units - 1) / r.units) + 1;
-    } else if (r.units < cus && r.units > 0) {
-      r.splits = (int)std::max<int64_t>(std::min<int64_t>(cus / r.units, tiles / kWaves), 1);
+    } else if (r.units < cus && r.units > 0 && tiles >= 4 * kWaves) {
+      r.splits = (int)std::min<int64_t>(cus / r.units, tiles / kWaves);
       if (r.splits > 1) pieces = r.units * r.splits;
       r.ways = r.splits;
     }
