@@ -633,12 +633,20 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   const int64_t span = p.window > 0 && p.window + rows < n.max_kv_len ? p.window + rows : n.max_kv_len;
   int cus = device_cus();
   if (cus <= 0) cus = 256;
-  // 16 rows to a column of the matrix instruction.  From 33 to 64 rows, two blocks of two columns while those leave compute
-  // units free and the cache is short (8 x 5 rows, group 7, window 4096: 31 us against the tile form's 36); otherwise the
-  // tile form (64 x 8 rows, group 5, 2048 tokens: 90 against 135 us; 1 x 60, 40 heads, 65536 tokens: 215 against 230).
-  const int64_t blocks2 = 2ll * n.batch * c.heads;
-  const bool few = blocks2 <= cus && blocks2 * span / kTileKeys < 64ll * cus;
-  r.nq = packed <= 16 ? 1 : packed <= 32 || (packed <= 64 && few) ? 2 : 0;
+  // Up to 16 rows are one column of the matrix instruction.  More go to the streaming form in blocks of two columns when
+  //  * one block has them all, or
+  //  * two do and no compute unit gets two blocks (16 x 40 rows, 8 heads, 1024 tokens: 17.5 us against the tile form's 29.2;
+  //    8 x 5, group 7, window 4096: 23 against 29) or the cache is long (24 x 9, group 4, 8192 tokens: 127 against 168 us;
+  //    64 x 8, group 5, 4096: 145 against 152; but 2048: 94 against 87, 512: 47 against 35), or
+  //  * any number does, no compute unit gets two, and either there are two for each block, so that it can be cut (1 x 160
+  //    rows, 12 heads, 8192 tokens: 29 against 38), or the cache is short (1 x 600, 12 heads, 2048 tokens: 25 against 41 us,
+  //    512: 14 against 25; 4 x 40, group 7, 3900: 36 against 43; but 1 x 100, 40 heads, 16384: 114 against 80).
+  // The rest is the tile form's, which loads a key once for 256 rows: at two blocks a compute unit it wins or draws (1 x
+  // 390, 30 heads, 2048 tokens: 42 against 43; 3900: 54 against 66).
+  const int64_t blocks = (packed + 31) / 32, wgs = blocks * n.batch * c.heads;
+  const bool stream = blocks <= 1 || (blocks <= 2 && (wgs <= cus || span >= 4096)) ||
+                      (wgs <= cus && (2 * wgs <= cus || span < 4096));
+  r.nq = packed <= 16 ? 1 : stream ? 2 : 0;
   r.block_rows = r.nq ? 16 * r.nq : kTileRows;
   r.nqb = (int)((packed + r.block_rows - 1) / r.block_rows);
   r.units = (int64_t)n.batch * c.heads * r.nqb;

@@ -741,3 +741,115 @@ def test_a_q_without_heads_does_not_keep_k_and_v_out(dev):
     assert all(torch.equal(a[n].view(torch.uint8), b[n].view(torch.uint8)) and torch.equal(a[n + "_scale"], b[n + "_scale"])
                for n in "kv")
     assert not torch.equal(a["k"].view(torch.uint8), c.host["k"].view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------------------------ the form for many rows
+
+class ManyRows(Case):
+    """The same batch under a bound on its rows that sends it to the form for many of them, with as many rows behind it."""
+
+    def __init__(self, dev, rows, lens, heads=2, group=1, **kw):
+        bound = 32 * 260 // (group * heads * len(rows)) + 64  # more blocks of 32 rows than compute units
+        kw["max_rows"] = max(bound, *rows)
+        super().__init__(dev, rows, lens, heads=heads, group=group, **kw)
+
+    def longer(self, q):
+        q = q.to(self.dev)
+        return torch.cat((q, torch.full((self.plan.max_rows, *q.shape[1:]), math.nan, dtype=BF, device=self.dev)))
+
+    def attend(self, q=None, **kw):
+        q = self.longer(self.q if q is None else q)
+        out = torch.full(q.shape, 7.0, dtype=BF, device=self.dev)
+        assert super().attend(q=q, out=out, **kw) is out
+        assert (out[self.total:] == 7).all()
+        return out[:self.total]
+
+
+@pytest.fixture
+def many_rows(monkeypatch):
+    monkeypatch.setitem(globals(), "Case", ManyRows)
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("kv", [1, 16, 63, 64, 65, 129, 777])
+def test_many_rows_one_token(dev, many_rows, page, kv):
+    check_attend(Case(dev, [1], [kv], page=page, seed=kv))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [0, 1, 33, 200])
+@pytest.mark.parametrize("page,group,rows,lens", [
+    (64, 1, [1, 3, 2], [100, 3, 260]),
+    (16, 7, [5, 1, 2, 4], [333, 2, 64, 4]),
+    (128, 4, [9, 4], [129, 500]),
+    (32, 1, [40, 17, 70], [50, 300, 70]),
+    (64, 2, [130, 1], [400, 31]),
+    (16, 1, [300], [300]),
+    (64, 3, [260], [520]),
+])
+def test_many_rows_ragged(dev, many_rows, page, group, rows, lens, window, causal):
+    check_attend(Case(dev, rows, lens, group=group, page=page, seed=sum(lens)), causal=causal, window=window)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows_that_see_nothing(dev, many_rows, causal):
+    test_rows_that_see_nothing_are_zero(dev, causal)
+
+
+def test_many_rows_scales_and_nan(dev, many_rows):
+    test_scales_far_apart_and_peaked_scores(dev)
+    test_nan_where_rows_do_not_look_stays_there(dev)
+    test_nan_and_infinite_queries_and_scales(dev)
+
+
+@pytest.mark.parametrize("rows,lens,window", [([5], [200], 0), ([150, 3], [200, 150], 40)])
+def test_many_rows_a_scale_of_nan(dev, many_rows, rows, lens, window):
+    test_a_scale_of_nan_reaches_only_rows_that_see_its_block(dev, rows, lens, window)
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("shape", ["rise", "fall", "spike", "late"])
+def test_many_rows_scores_that_move_the_reference(dev, many_rows, page, rows, shape):
+    test_scores_that_move_the_reference(dev, page, rows, shape)
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("rows,lens,heads,group,kw", [
+    ([300, 257], [9001, 4200], 7, 1, {}),  # page numbers loaded more than once
+    ([300], [9001], 14, 1, dict(causal=False, split_keys=False)),
+    ([300, 1], [9001, 8000], 7, 1, dict(window=5000)),
+    ([1100], [1100], 8, 1, {}),
+])
+def test_many_rows_long_key_ranges(dev, page, rows, lens, heads, group, kw):
+    test_long_key_ranges_and_forms_in_between(dev, page, rows, lens, heads, group, kw)
+
+
+def test_many_rows_bad_metadata(dev, many_rows):
+    for rows in ([2, 3, 1], [150, 10, 20]):
+        c = Case(dev, rows, [200, 190, 180], page=32, seed=41)
+        clean, s = c.attend(), c.starts
+        keep = c.plan.page_table[1, 2].clone()
+        for bad in (-5, 10 ** 9):
+            c.plan.page_table[1, 2] = bad
+            got = c.attend()
+            assert got[s[1]:s[2]].isnan().all()
+            assert torch.equal(got[:s[1]], clean[:s[1]]) and torch.equal(got[s[2]:], clean[s[2]:])
+        c.plan.page_table[1, 2] = keep
+        for bad in (-1, 201, 2 ** 31 - 1):
+            c.plan.kv_len[1] = bad
+            got = c.attend()
+            assert got[s[1]:s[2]].isnan().all()
+            assert torch.equal(got[:s[1]], clean[:s[1]]) and torch.equal(got[s[2]:], clean[s[2]:])
+        c.plan.kv_len[1] = 190
+        assert torch.equal(c.attend(), clean)
+
+
+@pytest.mark.parametrize("rows,lens", [([30], [700]), ([600], [900])])
+def test_many_rows_out_may_be_q(dev, many_rows, rows, lens):
+    from diffsynth_engine_amd import ops
+
+    c = Case(dev, rows, lens, group=3, seed=rows[0])
+    q = c.longer(c.q)
+    assert ops.kv_attention(q, c.cache, c.plan, out=q) is q
+    assert torch.equal(q[:c.total], c.attend()) and q[c.total:].isnan().all()
