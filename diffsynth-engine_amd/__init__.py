@@ -4,6 +4,7 @@ Public surface:
   attention.mi355x_attention / wan_attention / attention / set_attn_implementation
   fp8_linear.enable_fp8_linear / fp8_inference
   ops.*  (tensor-level wrappers of the C-ABI kernels in libdsx.so)
+  kv_cache.KVCache / KVPlan (a paged 8-bit key/value cache and a batch over it, for ops.kv_append / ops.kv_attention)
   flux_dit.FluxDiTRunner / wan_dit.WanDiTRunner (fused block runners), install.accelerate_flux_dit /
   accelerate_wan_dit (a runner behind a DiT module's forward), graph.GraphedStep (a step as a HIP graph)
 """

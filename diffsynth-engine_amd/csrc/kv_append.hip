@@ -3,7 +3,10 @@
 // One workgroup = one (page, head) block of K or of V, or 16 rows x kQHeads heads of q.  A block's tokens are held in
 // registers between the two passes over them (largest magnitude, then codes), so each element is read once and written
 // once: 16 lanes per token, 8 elements per lane, page/16 tokens per lane.  A row of q keeps its line of the rotation table in
-// registers for kQHeads heads.
+// registers for kQHeads heads (one head a row: 73 instead of 57 us at 8 x 2001 tokens).
+// Bound: HBM, 2 bytes in and 1 out an element of k and v, 2 and 2 of q.  8 x 2001 tokens, 8 heads, 32 of q: 57 us, 260 MB
+// (4.5 TB/s where a large copy reaches 4.9); 4680 tokens, 40 heads, without q: 30 us, 144 MB (4.7 TB/s); single tokens: the
+// launch, lengths, rows and the store in a row, 4.3 us.
 #include <stdlib.h>
 
 #include <algorithm>
