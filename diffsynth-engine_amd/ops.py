@@ -713,7 +713,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
     A block that keeps earlier tokens never lowers its scale; when it has to grow, the kept codes are rounded to the new
     one.  Infinities saturate, NaN stays NaN.  Appending the same rows at the same positions again changes nothing.
     A page must belong to one sequence while it is appended to.  Rows of a sequence that breaks a bound of the plan are
-    not appended (``plan.check`` finds them); rows behind the last sequence are left alone, in q_out too.
+    neither appended nor prepared (``plan.check`` finds them); they, and rows behind the last sequence, are left alone in
+    q_out.
 
     Returns q prepared (``q_out`` or a new tensor; q_out may be q), or None without q."""
     index = _kv_device("kv_append", cache, plan, k, v, q, q_out, k_norm_w, q_norm_w, rope)
@@ -767,9 +768,9 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     causal: row i of a sequence with r rows sees its first kv_len - r + i + 1 tokens; else all kv_len.  Of these only the
     last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive.
 
-    Rows of a sequence that breaks a bound of the plan become NaN, and so do rows that see a token whose page number is
-    out of range.  Rows of ``out`` behind the last sequence are left as they are (and hold nothing meaningful in an
-    ``out`` made here).  Where units of work are few, their key ranges are split over the chip through a workspace
+    Rows of a sequence that breaks a bound of the plan become NaN (the first plan.max_rows of them if there are more), and
+    so do rows that see a token whose page number is out of range.  Rows of ``out`` behind the last sequence are left as
+    they are (and hold nothing meaningful in an ``out`` made here).  Where units of work are few, their key ranges are split over the chip through a workspace
     allocated here (split_keys=False: never)."""
     index = _kv_device("kv_attention", cache, plan, q, out)
     if q.dim() != 3:
