@@ -15,12 +15,13 @@
 //    some of them would leave fp16 (2^15) does m become the maximum so far.  A tile that does not move it costs no
 //    rescaling of O, and where a tile has one scale (pages of 64 and more) no look at its scores' maximum either: the row
 //    sums, which are needed anyway, tell.
-// Bound: the matrix pipe with the vector work beside it: 2048 cycles of matrix instructions a tile and SIMD, 2156 of vector
-// instructions, 4062 measured.  4680 rows over 32760 tokens, 40 heads: 2.6 ms, 1210 TFLOP/s of the two products (a large
-// bf16 matrix product: 1525; the framework's attention over bf16 keys of the same size: 1125).  On that case, in copies
-// with work left out: without q's low term 8 % less, without exponentials 4 %, without V's conversion 5 %, without the
-// scores' maximum 7 % (of which looking at the row sums instead got 5).  Exponentials in other places (two to six in front
-// of the first product, 8 to 20 in the second stage): no change beyond noise.
+// Bound: the matrix pipe with the vector work and LDS beside it: 2048 cycles of matrix instructions a tile and SIMD, some 2100
+// of vector instructions, some 2100 of LDS, 3700 measured.  4680 rows over 32760 tokens, 40 heads: 2.40 ms, 1310 TFLOP/s of
+// the two products (a large bf16 matrix product: 1525; the framework's attention over bf16 keys of the same size: 1125).  On
+// that case (2.65 ms then), in copies with work left out: without q's low term 8 % less, without exponentials 4 %, without
+// V's conversion 5 %, without the scores' maximum 7 % (of which looking at the row sums instead got 5).  Exponentials in
+// other places (two to six in front of the first product, 8 to 20 in the second stage), three or four fragments of V ahead:
+// no change beyond noise.
 // LDS: K and V rows are 128 bytes; 16-byte piece j of K row r lies at j ^ (r & 7) (the permutation is applied to the
 // source address, the destination of a direct load being linear).
 #include "kv_attn_internal.h"
@@ -255,11 +256,13 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       const u32x4 y = *reinterpret_cast<const u32x4*>(smem + stage * kRaw + q * 2048 + (lane_k ^ 64));
       return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
-    auto v_frag = [&](int buf, int f) {
-      return *reinterpret_cast<const f16x8*>(smem + kOffVf + buf * kVf + f * 1024 + lane * 16);
-    };
-#define DSX_QK(S, Q, T, PART, ACC)                                                                          \
-  S[Q][T] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[T].PART, ACC, 0, 0, UNI ? 0 : Q, (int)ks, 0, qf[T].s_##PART)
+    // (one base for all of them: the offsets from the start of LDS are too long for the instruction's field, and each would
+    // be a sum of its own)
+    int lane_v = kOffVf + lane * 16;
+    asm volatile("" : "+v"(lane_v));
+    auto v_frag = [&](int buf, int f) { return *reinterpret_cast<const f16x8*>(smem + lane_v + (buf * kVf + f * 1024)); };
+#define DSX_QK(KF, Q, T, PART, ACC) \
+  __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(KF, qf[T].PART, ACC, 0, 0, UNI ? 0 : Q, (int)ks, 0, qf[T].s_##PART)
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
 
     // Position of the tile's key 4g in the row's span.  (Opaque: the differences of all 64 keys would be taken out of the
@@ -429,57 +432,49 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       if (more) scales_of(kb + 1, ks, vs);
       aim(kb + 3);
       DSX_HEAD(2);  // tile kb + 1 has landed, the fragments of V(kb) are written
+      // The two waves of a SIMD come here together, and of equal ones the first goes first: it was 900 of 3850 cycles early
+      // at the next barrier.  So the second leads in the first stage, and the first in the second.
+      if (wave >= 4) __builtin_amdgcn_s_setprio(1);
       {
         // ---- stage 1
         uint32_t raw[4];
         cv_read(st1, raw);
         if (__builtin_expect(boundary(kb + 1), 0)) cv_fix(kb + 1, buf ^ 1, raw);
-        i32x8 kf = k_frag(st1, 0), kn;
+        i32x8 kf[2] = {k_frag(st1, 0), k_frag(st1, 1)};
         f16x8 vf[kAhead + 1];
         int n = kExpEarly;
+        // Two 16-key groups at a time: their low terms for both columns, then their high terms, so that none waits for the
+        // product that it adds to.
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q < 3) kn = k_frag(st1, q + 1);
-          if (q == 3) {
+        for (int x = 0; x < 16; ++x) {
+          const int q = 2 * (x >> 3) + ((x >> 1) & 1), col = x & 1;
+          const bool high = (x >> 2) & 1;
+#define DSX_STEP(Q, T)                                                            \
+  if (q == Q && col == T) {                                                       \
+    if (high)                                                                     \
+      s_next[Q][T] = DSX_QK(kf[(Q) & 1], Q, T, hi, s_next[Q][T]);                 \
+    else                                                                          \
+      s_next[Q][T] = DSX_QK(kf[(Q) & 1], Q, T, lo, zero4);                        \
+  }
+          DSX_STEP(0, 0) DSX_STEP(0, 1) DSX_STEP(1, 0) DSX_STEP(1, 1) DSX_STEP(2, 0) DSX_STEP(2, 1) DSX_STEP(3, 0) DSX_STEP(3, 1)
+#undef DSX_STEP
+          // (pinned: nothing in front of the next branch needs the products, and they would be sunk behind it, away from the
+          // vector work that is to run beside them)
+          if (high) asm volatile("" : "+v"(s_next[q][col]));
+          if (x == 5) kf[0] = k_frag(st1, 2);
+          if (x == 7) kf[1] = k_frag(st1, 3);
+          if (x == 12) {
 #pragma unroll
             for (int f = 0; f < kAhead; ++f) vf[f] = v_frag(buf, f);
           }
+          // 32 - kExpEarly entries spread over 16 slots
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {  // the two columns' low terms, then their high terms
-            if (x == 0) {
-              if (q == 0) DSX_QK(s_next, 0, 0, lo, zero4);
-              if (q == 1) DSX_QK(s_next, 1, 0, lo, zero4);
-              if (q == 2) DSX_QK(s_next, 2, 0, lo, zero4);
-              if (q == 3) DSX_QK(s_next, 3, 0, lo, zero4);
-            } else if (x == 1) {
-              if (q == 0) DSX_QK(s_next, 0, 1, lo, zero4);
-              if (q == 1) DSX_QK(s_next, 1, 1, lo, zero4);
-              if (q == 2) DSX_QK(s_next, 2, 1, lo, zero4);
-              if (q == 3) DSX_QK(s_next, 3, 1, lo, zero4);
-            } else if (x == 2) {
-              if (q == 0) DSX_QK(s_next, 0, 0, hi, s_next[0][0]);
-              if (q == 1) DSX_QK(s_next, 1, 0, hi, s_next[1][0]);
-              if (q == 2) DSX_QK(s_next, 2, 0, hi, s_next[2][0]);
-              if (q == 3) DSX_QK(s_next, 3, 0, hi, s_next[3][0]);
-            } else {
-              if (q == 0) DSX_QK(s_next, 0, 1, hi, s_next[0][1]);
-              if (q == 1) DSX_QK(s_next, 1, 1, hi, s_next[1][1]);
-              if (q == 2) DSX_QK(s_next, 2, 1, hi, s_next[2][1]);
-              if (q == 3) DSX_QK(s_next, 3, 1, hi, s_next[3][1]);
-            }
-            // (pinned: nothing in front of the next branch needs the products, and they would be sunk behind it, away from the
-            // vector work that is to run beside them)
-            if (x >= 2) asm volatile("" : "+v"(s_next[q][x - 2]));
-            // 32 - kExpEarly entries spread over 16 slots
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-              if ((n - kExpEarly) * 16 < (4 * q + x + 1) * (32 - kExpEarly)) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
-            if (q == 1 && x == 0) issue_k(st3);
-            if (q == 1 && x == 2) cv_write(buf ^ 1, raw);
-            if (q == 2 && x == 2) issue_v(st3);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          if (q < 3) kf = kn;
+          for (int y = 0; y < 2; ++y)
+            if ((n - kExpEarly) * 16 < (x + 1) * (32 - kExpEarly)) exp_entry(s_cur, off_cur, inv_cur, pw_cur, n++);
+          if (x == 4) issue_k(st3);
+          if (x == 6) cv_write(buf ^ 1, raw);
+          if (x == 10) issue_v(st3);
+          __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (UNI) {
           // A lane's sum over its keys bounds each of its weights: as long as it fits fp16, so do they, and the scores' own
@@ -502,6 +497,7 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
           lsum[t] = 0.f;
         }
         // ---- stage 2
+        if (wave >= 4) __builtin_amdgcn_s_setprio(0);
         float ev[kGroups];
         scale_floats(vs, ev, inv_next);
         auto pv = [&](int f, int t) {
@@ -563,12 +559,12 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       cv_write(0, raw);
       if (active) {
         i32x8 kf;
-#define DSX_FIRST(Q)                     \
-  kf = k_frag(0, Q);                     \
-  DSX_QK(sA, Q, 0, lo, zero4);           \
-  DSX_QK(sA, Q, 1, lo, zero4);           \
-  DSX_QK(sA, Q, 0, hi, sA[Q][0]);        \
-  DSX_QK(sA, Q, 1, hi, sA[Q][1]);
+#define DSX_FIRST(Q)                                 \
+  kf = k_frag(0, Q);                                 \
+  sA[Q][0] = DSX_QK(kf, Q, 0, lo, zero4);            \
+  sA[Q][1] = DSX_QK(kf, Q, 1, lo, zero4);            \
+  sA[Q][0] = DSX_QK(kf, Q, 0, hi, sA[Q][0]);         \
+  sA[Q][1] = DSX_QK(kf, Q, 1, hi, sA[Q][1]);
         DSX_FIRST(0) DSX_FIRST(1) DSX_FIRST(2) DSX_FIRST(3)
 #undef DSX_FIRST
         float ev[kGroups], mx[2];
