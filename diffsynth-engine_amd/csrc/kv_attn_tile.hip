@@ -422,15 +422,13 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     uint32_t pwA[2][2][4], pwB[2][2][4];
     float offA[kGroups][2], offB[kGroups][2], invA[kGroups], invB[kGroups];
 
+    uint32_t ks, vs;  // scales of tile kb + 1
     auto interval = [&](int kb, int buf, f32x4 (&s_cur)[4][2], f32x4 (&s_next)[4][2], uint32_t (&pw_cur)[2][2][4],
                         uint32_t (&pw_next)[2][2][4], float (&off_cur)[kGroups][2],
                         const float (&inv_cur)[kGroups], float (&off_next)[kGroups][2], float (&inv_next)[kGroups]) __attribute__((always_inline)) {
       const int i = kb - kb_begin;
       const int st1 = (i + 1) & 3, st3 = (i + 3) & 3;
       const bool more = kb + 1 < kb_end;
-      uint32_t ks = 0x7f7f7f7fu, vs = 0x7f7f7f7fu;
-      if (more) scales_of(kb + 1, ks, vs);
-      aim(kb + 3);
       DSX_HEAD(2);  // tile kb + 1 has landed, the fragments of V(kb) are written
       // The two waves of a SIMD come here together, and of equal ones the first goes first: it was 900 of 3850 cycles early
       // at the next barrier.  So the second leads in the first stage, and the first in the second.
@@ -531,6 +529,9 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             pv(f, t);
+            // for the next interval: scalar work, which at its head would have nothing beside it
+            if (f == 5 && t == 0) scales_of(kb + 2, ks, vs);
+            if (f == 9 && t == 0) aim(kb + 4);
             // kExpEarly entries spread over the slots that are left
             if (n2 * 2 * (16 - kScanFrags) < (2 * (f - kScanFrags) + t + 1) * kExpEarly)
               exp_entry(s_next, off_next, inv_next, pw_next, n2++);
@@ -549,7 +550,6 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
     aim(kb_begin + 2);
     issue_k(2);
     issue_v(2);
-    uint32_t ks, vs;
     scales_of(kb_begin, ks, vs);
     DSX_HEAD(4);
     {
@@ -590,6 +590,8 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
         cv_write((i + 1) & 1, raw);
       }
     }
+    scales_of(kb_begin + 1, ks, vs);
+    aim(kb_begin + 3);
     for (int kb = kb_begin; active && kb < kb_end; kb += 2) {
       interval(kb, 0, sA, sB, pwA, pwB, offA, invA, offB, invB);
       if (kb + 1 < kb_end) interval(kb + 1, 1, sB, sA, pwB, pwA, offB, invB, offA, invA);
