@@ -16,7 +16,7 @@
 //    rescaling of O, and where a tile has one scale (pages of 64 and more) no look at its scores' maximum either: the row
 //    sums, which are needed anyway, tell.
 // Bound: the matrix pipe with the vector work and LDS beside it: 2048 cycles of matrix instructions a tile and SIMD, some 2100
-// of vector instructions, some 2100 of LDS, 3700 measured.  4680 rows over 32760 tokens, 40 heads: 2.40 ms, 1310 TFLOP/s of
+// of vector instructions, some 2100 of LDS, 3600 measured.  4680 rows over 32760 tokens, 40 heads: 2.40 ms, 1310 TFLOP/s of
 // the two products (a large bf16 matrix product: 1525; the framework's attention over bf16 keys of the same size: 1125).  On
 // that case (2.65 ms then), in copies with work left out: without q's low term 8 % less, without exponentials 4 %, without
 // V's conversion 5 %, without the scores' maximum 7 % (of which looking at the row sums instead got 5).  Exponentials in
