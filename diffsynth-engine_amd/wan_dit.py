@@ -57,7 +57,8 @@ def wan_config_from_shapes(shapes: Dict[str, tuple], eps: float = 1e-6) -> dict:
 
 class WanFrameCache:
     """Self-attention keys and values of a video's frames so far, 8 bits wide, one ``KVCache`` per block of the model
-    (``WanDiTRunner.frame_cache`` makes it).  ``frames``: how many frames (in tokens' time steps) it holds."""
+    (``WanDiTRunner.frame_cache`` makes it).  ``frames``: how many frames (in tokens' time steps) it holds.  Keys and
+    values depend on the prompt: each guidance branch needs a cache of its own, or its entry of the batch."""
 
     def __init__(self, layers: int, heads: int, frames: int, h: int, w: int, batch: int, page_size: int, device):
         if min(layers, heads, frames, h, w, batch) < 1:
@@ -239,7 +240,8 @@ class WanDiTRunner:
         ``cache``: x holds the latent frames [first_frame, first_frame + x.shape[2]) of a longer video.  They attend to
         one another and to the frames in front of them, as the cache has them; their own keys and values replace what it
         holds from first_frame on.  A denoising loop calls this with the same first_frame for every step of a run of
-        frames, and goes on behind them when they are done."""
+        frames, and goes on behind them when they are done; what stays in the cache is the last call's, so whoever wants
+        the finished frames there, and not those of the last noisy step, calls once more with them."""
         cfg = self.cfg
         d = cfg["dim"]
         pf, ph, pw = cfg["patch_size"]
