@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_stream_kernel(AttnArgs a) {
     const int unit = a.by_splits(blockIdx.x);
     kv_unit(a, unit, b, h, qb);
     b = uniform(b);
-    if (a.splits > 1) {
+    if (a.splits > 1) {  // a piece takes every a.splits-th run of eight tiles: its first page needs no length
       first += kWaves * (int)(blockIdx.x - unit * a.splits);
       stride *= a.splits;
       piece = blockIdx.x;
