@@ -28,7 +28,7 @@ from typing import Dict, Optional
 import torch
 
 from . import ops
-from .kv_cache import KVCache, KVPlan
+from .kv_cache import E4M3, E8M0, PAGE_SIZES, KVCache, KVPlan
 from .flux_dit import _Linear, _gemm_pair, count_blocks, ingest_state_dict
 
 
@@ -58,15 +58,30 @@ def wan_config_from_shapes(shapes: Dict[str, tuple], eps: float = 1e-6) -> dict:
 class WanFrameCache:
     """Self-attention keys and values of a video's frames so far, 8 bits wide, one ``KVCache`` per block of the model
     (``WanDiTRunner.frame_cache`` makes it).  ``frames``: how many frames (in tokens' time steps) it holds.  Keys and
-    values depend on the prompt: each guidance branch needs a cache of its own, or its entry of the batch."""
+    values depend on the prompt: each guidance branch needs a cache of its own, or its entry of the batch.
+
+    A run of frames whose first token lies inside a page shares that page's scales with finished tokens, and an append
+    never lowers a scale.  The cache therefore keeps a copy of that page of every block from before the run and begins
+    each further step of the run with it: what a step leaves is what it alone would have left, whatever the steps before
+    it wrote."""
 
     def __init__(self, layers: int, heads: int, frames: int, h: int, w: int, batch: int, page_size: int, device):
         if min(layers, heads, frames, h, w, batch) < 1:
             raise ValueError("WanFrameCache: every size must be at least 1")
+        if page_size not in PAGE_SIZES:
+            raise ValueError("WanFrameCache: page_size must be one of %s" % (PAGE_SIZES,))
         self.max_frames, self.h, self.w, self.batch, self.frames = frames, h, w, batch, 0
+        self.page_size = page_size
         pages = -(-frames * h * w // page_size)
-        self.layers = [KVCache.empty(batch * pages, heads, page_size, device) for _ in range(layers)]
+        # keys and values of every block in one tensor: a page of all of them is one strided copy
+        self._codes = torch.zeros((2, layers, batch, pages, heads, page_size, 128), dtype=torch.uint8, device=device)
+        self._scales = torch.full((2, layers, batch, pages, heads), 127, dtype=torch.uint8, device=device)
+        k, v = self._codes.flatten(2, 3).view(E4M3)
+        ks, vs = self._scales.flatten(2, 3).view(E8M0)
+        self.layers = [KVCache(k[i], v[i], ks[i], vs[i]) for i in range(layers)]
         self.table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
+        self._before = {}     # first frame of a run -> its first page as it was before the run
+        self._begun = set()   # the runs whose copy is up to date
 
     def bytes(self) -> int:
         return sum(t.numel() for c in self.layers for t in (c.k, c.v, c.k_scale, c.v_scale))
@@ -80,6 +95,30 @@ class WanFrameCache:
         starts = torch.arange(0, (self.batch + 1) * rows, rows, dtype=torch.int32, device=self.table.device)
         lens = torch.full((self.batch,), tokens, dtype=torch.int32, device=self.table.device)
         return KVPlan(self.table, starts, lens, max_rows=rows, max_kv_len=tokens)
+
+    def step(self, first: int, frames: int) -> KVPlan:
+        """``plan``, with the page that the run begins in as it was before the run's first step.  Going back into the
+        middle of an earlier run makes that point a run of its own, from the page as it is then.  The first step of a run
+        that begins inside a page cannot be recorded into a graph (its replays would copy what they wrote themselves);
+        later ones can, and replays are good for as long as the run is the newest."""
+        plan = self.plan(first, frames)
+        page, kept = divmod(first * self.h * self.w, self.page_size)
+        if kept:
+            now = self._codes[:, :, :, page], self._scales[:, :, :, page]
+            if first in self._begun:
+                for t, saved in zip(now, self._before[first]):
+                    t.copy_(saved)
+            else:
+                if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("WanFrameCache: the first step of a run that begins inside a page cannot be "
+                                       "recorded into a graph; run one step before")
+                if first in self._before:  # (never given back while a recorded step may read it)
+                    for t, saved in zip(now, self._before[first]):
+                        saved.copy_(t)
+                else:
+                    self._before[first] = tuple(t.clone() for t in now)
+        self._begun = {n for n in self._begun if n < first} | {first}
+        return plan
 
 
 class WanDiTRunner:
@@ -239,7 +278,7 @@ class WanDiTRunner:
 
         ``cache``: x holds the latent frames [first_frame, first_frame + x.shape[2]) of a longer video.  They attend to
         one another and to the frames in front of them, as the cache has them; their own keys and values replace what it
-        holds from first_frame on.  A denoising loop calls this with the same first_frame for every step of a run of
+        holds from first_frame on, as if no step before had written there.  A denoising loop calls this with the same first_frame for every step of a run of
         frames, and goes on behind them when they are done; what stays in the cache is the last call's, so whoever wants
         the finished frames there, and not those of the last noisy step, calls once more with them."""
         cfg = self.cfg
@@ -272,7 +311,7 @@ class WanDiTRunner:
                 raise ValueError("the cache was made for a batch of %d, %d x %d tokens a frame and %d blocks"
                                  % (cache.batch, cache.h, cache.w, len(cache.layers)))
             first = first_frame // pf
-            plan = cache.plan(first, f)
+            plan = cache.step(first, f)
         patches = x.to(bf).view(B, C, f, pf, h, ph, w, pw).permute(0, 2, 4, 6, 1, 3, 5, 7)
         hs = self._linear_bf16(patches.reshape(B, f * h * w, C * pf * ph * pw), "patch_embedding")
         rope = self.rope_table(f, h, w, first=first)
