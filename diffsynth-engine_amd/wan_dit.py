@@ -316,6 +316,8 @@ class WanDiTRunner:
         hs = self._linear_bf16(patches.reshape(B, f * h * w, C * pf * ph * pw), "patch_embedding")
         rope = self.rope_table(f, h, w, first=first)
         ctx_q = self.quantise_context(ctx)
+        if cache is not None:
+            cache.frames = first  # (should a block raise: what was there from here on is overwritten in part)
         for i in range(cfg["num_layers"]):
             hs = self.block(i, hs, ctx, t_mod, rope, ctx_q, None if cache is None else (cache.layers[i], plan))
         if cache is not None:

@@ -74,3 +74,27 @@ def test_recorded_steps(dev):
         torch.cuda.synchronize()
         assert torch.equal(step(x=y), want), i
         assert all(torch.equal(a, b) for a, b in zip(_state(eager), _state(replayed)))
+
+
+def test_a_step_that_raises_leaves_no_frames_that_it_overwrote(dev, monkeypatch):
+    R = _runner(dev)
+    x, ctx, t = _inputs(dev, 3)
+    cache, twin = (R.frame_cache(3, 12, 14) for _ in range(2))
+    for c in (cache, twin):
+        R(x, ctx, t, cache=c)
+    block = R.block
+
+    def stops(i, *args, **kw):
+        if i == 1:
+            raise KeyboardInterrupt
+        return block(i, *args, **kw)
+
+    part = x[:, :, 1:2].contiguous()
+    monkeypatch.setattr(R, "block", stops)
+    with pytest.raises(KeyboardInterrupt):
+        R(part, ctx, t, cache=cache, first_frame=1)
+    monkeypatch.undo()
+    assert cache.frames == 1
+    with pytest.raises(ValueError):  # frame 1 is not there any more
+        R(x[:, :, 2:].contiguous(), ctx, t, cache=cache, first_frame=2)
+    assert torch.equal(R(part, ctx, t, cache=cache, first_frame=1), R(part, ctx, t, cache=twin, first_frame=1))
