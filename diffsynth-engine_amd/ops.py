@@ -666,6 +666,37 @@ def _kv_apart(name: str, rows: int, heads: int, sr: int, sh: int):
         raise ValueError("%s: its elements overlap in memory" % name)
 
 
+def _kv_meet(a, b) -> bool:
+    """Whether two (rows, heads, 128) views, each (pointer, row stride, head stride, rows, heads), share an element."""
+    (pa, ra, ha, na, ma), (pb, rb, hb, nb, mb) = a, b
+    len_a, len_b = (ma - 1) * ha + HEAD_DIM, (mb - 1) * hb + HEAD_DIM  # elements of a row, with what lies between heads
+    d = (pb - pa) // 2
+    if d >= (na - 1) * ra + len_a or -d >= (nb - 1) * rb + len_b or not (na and ma and nb and mb):
+        return False
+    if ra == rb and len_a <= ra and len_b <= ra:  # columns of one packed projection
+        at = d % ra
+        if at >= len_a and at + len_b <= ra:
+            return False
+    # heads of one view between those of the other: every 128 elements by themselves
+    starts = [(torch.arange(n)[:, None] * r + torch.arange(m) * h).flatten().sort().values
+              for _, r, h, n, m in (a, b)]
+    where = torch.searchsorted(starts[0], starts[1] + (d - HEAD_DIM), right=True).clamp(max=len(starts[0]) - 1)
+    return bool(((starts[0][where] - starts[1] - d).abs() < HEAD_DIM).any())
+
+
+def _kv_out_clear(name: str, out, source, *others):
+    """`out` may be `source` itself, element for element, and must share nothing with it otherwise, nor with the others:
+    the kernels read them while they write it."""
+    if out != source:
+        po, ro, ho, n, m = out
+        ps, rs, hs, _, _ = source
+        if not (po == ps and (ro == rs or n < 2) and (ho == hs or m < 2)) and _kv_meet(out, source):
+            raise ValueError("%s overlaps an input in memory" % name)
+    for x in others:
+        if _kv_meet(out, x):
+            raise ValueError("%s overlaps an input in memory" % name)
+
+
 def _kv_device(name: str, cache: KVCache, plan: KVPlan, *tensors) -> int:
     """The one device that everything is on (a number: these calls are short, and device objects take a while)."""
     index = plan._index
@@ -716,7 +747,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
     neither appended nor prepared (``plan.check`` finds them); they, and rows behind the last sequence, are left alone in
     q_out.
 
-    Returns q prepared (``q_out`` or a new tensor; q_out may be q), or None without q."""
+    Returns q prepared (``q_out`` or a new tensor; q_out may be q itself, and shares no memory with q, k or v otherwise),
+    or None without q."""
     index = _kv_device("kv_append", cache, plan, k, v, q, q_out, k_norm_w, q_norm_w, rope)
     if k.dim() != 3:
         raise ValueError("kv_append: k must be (rows, heads, 128)")
@@ -739,6 +771,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
         else:
             qop, qo_sr, qo_sh = _kv_rows("kv_append: q_out", q_out, rows, heads)
             _kv_apart("kv_append: q_out", rows, heads, qo_sr, qo_sh)
+            _kv_out_clear("kv_append: q_out", (qop, qo_sr, qo_sh, rows, heads), (qp, q_sr, q_sh, rows, heads),
+                          (kp, k_sr, k_sh, rows, cache.heads), (vp, v_sr, v_sh, rows, cache.heads))
     if k_norm_w is not None:
         k_norm_w = _kv_norm_weight(k_norm_w)
     if q_norm_w is not None:
@@ -764,7 +798,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     """softmax(q k^T * scale) v of packed rows over the tokens their sequences have in a paged 8-bit cache.
 
     q, out: (rows, heads, 128) bf16, heads a multiple of cache.heads (query head h reads cache head
-    h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8; out may be q.
+    h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8; out may be q
+    itself, and shares no memory with it otherwise.
     causal: row i of a sequence with r rows sees its first kv_len - r + i + 1 tokens; else all kv_len.  Of these only the
     last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive.
 
@@ -790,6 +825,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     else:
         op, o_sr, o_sh = _kv_rows("kv_attention: out", out, rows, heads)
         _kv_apart("kv_attention: out", rows, heads, o_sr, o_sh)
+        _kv_out_clear("kv_attention: out", (op, o_sr, o_sh, rows, heads), (qp, q_sr, q_sh, rows, heads))
     if not rows:
         return out
     lib = _lib.load()

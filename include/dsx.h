@@ -416,7 +416,8 @@ typedef struct dsx_kv_batch {
  * Appends a batch's rows to the cache and prepares its queries, one launch:
  *   k: RMSNorm over the head (k_norm_w bf16 (128,), NULL = none), rotation of the pairs (2i, 2i+1) by the (cos, sin) of
  *      table row `position` (rope NULL = none), block scale, e4m3;   v: block scale, e4m3;
- *   q (NULL = none): RMSNorm (q_norm_w), rotation, bf16 to q_out (which may be q itself).
+ *   q (NULL = none): RMSNorm (q_norm_w), rotation, bf16 to q_out (which may be q itself, and otherwise
+ *      shares no memory with q, k or v).
  * A row's position is its token number in its sequence.  fp32 throughout, rounded once where it is stored (the row
  * kernels dsx_rmsnorm_rope* round to bf16 in between).
  * Block scale: with a the largest finite magnitude among the block's new tokens, e = the smallest integer in [-48, 48]
@@ -448,7 +449,8 @@ int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const ds
  * Query head h reads cache head h / (heads_q / heads); heads_q is a multiple of heads.
  * Softmax and sums in fp32.  q is used as the exact sum of two scaled e4m3 terms (each element to 2^-22 of its row's
  * largest), the weights enter the second product as fp16.  A q row with a non-finite element gives NaN.
- * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned); out may be q.
+ * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned); out may be q
+ * itself, and otherwise shares no memory with it.
  * workspace: dsx_kv_attn_workspace_bytes(...) bytes, 16-byte aligned, lets the key range be split over the compute units
  * and the pieces be joined by a second launch; NULL: never split.  Calls that share a workspace must not overlap.
  */

@@ -1,0 +1,110 @@
+"""What ops.kv_append and ops.kv_attention refuse, and what they hand to the library, on the host: the device is replaced
+by host tensors and the library by one that writes down its calls."""
+import contextlib
+import itertools
+import random
+
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+class Recorder:
+    """Stands in for the library: every function notes the current device and returns 0."""
+
+    def __init__(self):
+        self.calls = []
+        self.device = 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, self.device))
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """ops with host tensors that pass for device 1's while device 0 is current."""
+    from diffsynth_engine_amd import _lib, ops
+
+    rec = Recorder()
+
+    @contextlib.contextmanager
+    def on(index):
+        old, rec.device = rec.device, index
+        yield
+        rec.device = old
+
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(ops, "_kv_device", lambda *a: 1)
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: rec.device, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    return rec
+
+
+def _batch(heads=2, rows=6):
+    from diffsynth_engine_amd.kv_cache import KVCache, KVPlan
+
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return (KVCache.empty(4, heads, 16, "cpu"),
+            KVPlan(torch.arange(4, dtype=torch.int32)[None], i32(0, rows), i32(40), max_rows=rows, max_kv_len=64))
+
+
+def _elements(view):
+    return set((view.data_ptr() // 2 + i * view.stride(0) + j * view.stride(1) + e)
+               for i in range(view.shape[0]) for j in range(view.shape[1]) for e in range(128))
+
+
+def test_views_meet_where_their_elements_do():
+    from diffsynth_engine_amd.ops import _kv_meet
+
+    r = random.Random(3)
+    buf = torch.empty(60000, dtype=BF)
+    seen = {True: 0, False: 0}
+    for _ in range(400):
+        views = []
+        for _ in range(2):
+            rows, heads = r.randrange(1, 6), r.randrange(1, 5)
+            sh = r.choice((128, 128, 136, 256, 384, 1280))
+            sr = r.choice((128 * heads, 1280, 1280, 640, 128, 2560, 1288))
+            at = 8 * r.randrange(0, 700)
+            views.append(buf.as_strided((rows, heads, 128), (sr, sh, 1), at))
+        for a, b in (views, views[::-1]):
+            got = _kv_meet(*((t.data_ptr(), t.stride(0), t.stride(1), *t.shape[:2]) for t in (a, b)))
+            assert got == bool(_elements(a) & _elements(b)), (a.shape, a.stride(), b.shape, b.stride())
+            seen[got] += 1
+    assert min(seen.values()) > 100
+    for shape in ((0, 3, 128), (3, 0, 128)):
+        t = buf.as_strided(shape, (384, 128, 1))
+        assert not _kv_meet(*((t.data_ptr(), 384, 128, *shape[:2]) for _ in range(2)))
+
+
+def test_outputs_over_inputs_are_refused(calls):
+    from diffsynth_engine_amd import ops
+
+    cache, plan = _batch()
+    packed = torch.zeros(8, 8, 128, dtype=BF)
+    q, k, v = packed[:6, :4], packed[:6, 4:6], packed[:6, 6:]
+    row_on, head_on = packed[1:7, :4], packed[:6, 1:5]
+    far = torch.empty_like(packed)
+    for bad in (row_on, head_on):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.kv_attention(q, cache, plan, out=bad)
+    for bad in (row_on, head_on, packed[:6, 2:6], packed[:6, 4:], packed[2:, 3:7]):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.kv_append(k, v, cache, plan, q=q, q_out=bad)
+    with pytest.raises(ValueError, match="overlaps"):  # q itself, but k is a part of it
+        ops.kv_append(q[:, 1:3], v, cache, plan, q=q, q_out=q)
+    assert not calls.calls
+    for good in (q, far[:6, :4], far[2:, 1:5], far[:6, ::2]):
+        assert ops.kv_attention(q, cache, plan, out=good) is good
+        assert ops.kv_append(k, v, cache, plan, q=q, q_out=good) is good
+    assert ops.kv_attention(q, cache, plan, out=packed[:6, 4:]) is not None  # what is not read here may be written
+    wide = torch.zeros(6, 8, 128, dtype=BF)
+    for a, b in itertools.permutations((wide[:, ::2], wide[:, 1::2])):  # every other head of one buffer
+        assert ops.kv_attention(a, cache, plan, out=b) is b
+    one = wide[:1, :1]
+    assert ops.kv_attention(one, _batch(1, 1)[0], plan, out=one.as_strided((1, 1, 128), (8, 8, 1))) is not None
