@@ -630,7 +630,7 @@ int check(const dsx_kv_cache* c, const dsx_kv_batch* n, const dsx_kv_attn_params
   const int rc = kv_check_cache(c, n, p->total_rows);
   if (rc != DSX_OK) return rc;
   if (p->heads_q < 1 || p->heads_q % c->heads || p->window < 0) return DSX_EBADSHAPE;
-  if (!(p->softmax_scale > 0.f) || !(p->softmax_scale < INFINITY)) return DSX_EBADSHAPE;
+  if (!(p->softmax_scale > 0.f) || !(p->softmax_scale * kLog2e < INFINITY)) return DSX_EBADSHAPE;
   if ((int64_t)n->max_rows * (p->heads_q / c->heads) > (1 << 30)) return DSX_EBADSHAPE;
   return DSX_OK;
 }

@@ -801,7 +801,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     h // (heads // cache.heads)); unit stride in the last dim, other strides in multiples of 8; out may be q
     itself, and shares no memory with it otherwise.
     causal: row i of a sequence with r rows sees its first kv_len - r + i + 1 tokens; else all kv_len.  Of these only the
-    last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive.
+    last ``window`` when that is not 0.  A row that sees nothing gives zeros.  scale: 1/sqrt(128) by default, positive, below
+    2.3e38 (the kernels work with scale * log2 e).
 
     Rows of a sequence that breaks a bound of the plan become NaN (the first plan.max_rows of them if there are more), and
     so do rows that see a token whose page number is out of range.  Rows of ``out`` behind the last sequence are left as
@@ -817,8 +818,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     if window < 0 or window > 0x7fffffff:
         raise ValueError("kv_attention: window must lie in [0, 2^31)")
     scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError("kv_attention: scale must be positive and finite")
+    if not 0.0 < scale < 2.3e38:
+        raise ValueError("kv_attention: scale must be positive and below 2.3e38")
     if out is None:
         out = q.new_empty((rows, heads, HEAD_DIM))
         op, o_sr, o_sh = out.data_ptr(), heads * HEAD_DIM, HEAD_DIM

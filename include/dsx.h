@@ -458,7 +458,7 @@ typedef struct dsx_kv_attn_params {
   const void* q; int64_t q_sr, q_sh;
   void* out; int64_t o_sr, o_sh;
   int64_t total_rows;                /* rows that q and out have */
-  float softmax_scale;               /* > 0 */
+  float softmax_scale;               /* > 0, softmax_scale * log2(e) finite */
   int32_t heads_q, causal, window;
   void* workspace; int64_t workspace_bytes;
 } dsx_kv_attn_params;

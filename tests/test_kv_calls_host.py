@@ -108,3 +108,30 @@ def test_outputs_over_inputs_are_refused(calls):
         assert ops.kv_attention(a, cache, plan, out=b) is b
     one = wide[:1, :1]
     assert ops.kv_attention(one, _batch(1, 1)[0], plan, out=one.as_strided((1, 1, 128), (8, 8, 1))) is not None
+
+
+def test_a_scale_whose_base_2_form_is_infinite_is_refused(calls):
+    # fp32's largest number over log2(e) is 2.36e38: beyond it 0 * infinity made NaN of a score of zero
+    from diffsynth_engine_amd import ops
+
+    cache, plan = _batch()
+    q = torch.zeros(6, 2, 128, dtype=BF)
+    for bad in (2.3e38, 2.9e38):
+        with pytest.raises(ValueError, match="scale"):
+            ops.kv_attention(q, cache, plan, scale=bad)
+    assert not calls.calls
+    ops.kv_attention(q, cache, plan, scale=2.2e38)
+
+
+def test_the_library_refuses_it_too():
+    import ctypes
+
+    from diffsynth_engine_amd import _lib
+
+    cache, plan = _batch()
+    for scale, need in ((2.3e38, True), (2.4e38, False), (3.4e38, False)):
+        P = _lib.KVAttnParams(total_rows=6, softmax_scale=scale, heads_q=2)
+        long = type(plan._c).from_buffer_copy(plan._c)
+        long.max_kv_len, long.table_pages, long.table_sb = 1 << 20, 1 << 16, 1 << 16
+        got = _lib.load().dsx_kv_attn_workspace_bytes(ctypes.byref(cache._c), ctypes.byref(long), ctypes.byref(P))
+        assert (got > 0) == need  # (0 for a call that would be refused)
