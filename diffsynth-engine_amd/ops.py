@@ -832,9 +832,13 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     lib = _lib.load()
     p = _lib.KVAttnParams(qp, q_sr, q_sh, op, o_sr, o_sh, rows, scale, heads, bool(causal), window, None, 0)
     ref = ctypes.byref(p)
-    need = lib.dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, ref) if split_keys else 0
-    if need > 0:
-        ws = q.new_empty(need // 2)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), need
-    _kv_call(lib.dsx_kv_attn, "dsx_kv_attn", index, cache._ref, plan._ref, ref)
+
+    def launch(c, n, ref, stream):
+        need = lib.dsx_kv_attn_workspace_bytes(c, n, ref) if split_keys else 0  # (asks the current device for its size)
+        if need > 0:
+            ws = q.new_empty(need // 2)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        return lib.dsx_kv_attn(c, n, ref, stream)
+
+    _kv_call(launch, "dsx_kv_attn", index, cache._ref, plan._ref, ref)
     return out

@@ -135,3 +135,15 @@ def test_the_library_refuses_it_too():
         long.max_kv_len, long.table_pages, long.table_sb = 1 << 20, 1 << 16, 1 << 16
         got = _lib.load().dsx_kv_attn_workspace_bytes(ctypes.byref(cache._c), ctypes.byref(long), ctypes.byref(P))
         assert (got > 0) == need  # (0 for a call that would be refused)
+
+
+def test_the_workspace_is_sized_by_the_tensors_device(calls):
+    # how a call is split depends on the compute units of the device that it runs on
+    from diffsynth_engine_amd import ops
+
+    cache, plan = _batch()
+    ops.kv_attention(torch.zeros(6, 2, 128, dtype=BF), cache, plan)
+    assert calls.calls == [("dsx_kv_attn_workspace_bytes", 1), ("dsx_kv_attn", 1)] and calls.device == 0
+    calls.calls.clear()
+    ops.kv_attention(torch.zeros(6, 2, 128, dtype=BF), cache, plan, split_keys=False)
+    assert calls.calls == [("dsx_kv_attn", 1)]
