@@ -19,6 +19,7 @@ E4M3 = torch.float8_e4m3fn
 E8M0 = torch.float8_e8m0fnu
 HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
+EXPONENTS = (-48, 48)  # of a block's scale
 
 
 class _Fixed:
@@ -39,8 +40,9 @@ def _apart(shape, strides, inner: int) -> bool:
 
 class KVCache(_Fixed):
     """Codes ``k``, ``v``: (pages, heads, page_size, 128) e4m3, any page and head strides that are multiples of 16, each
-    (page, head) block contiguous.  Scales ``k_scale``, ``v_scale``: (pages, heads) e8m0, heads contiguous.  A value is
-    code * scale.  The tensors stay the caller's and are used in place; which they are is fixed when the cache is made."""
+    (page, head) block contiguous.  Scales ``k_scale``, ``v_scale``: (pages, heads) e8m0, heads contiguous, from 2^-48 to
+    2^48 (or NaN) wherever a token lies: others give inexact results, and nothing but ``KVPlan.check`` looks for them.  A
+    value is code * scale.  The tensors stay the caller's and are used in place; which they are is fixed when the cache is made."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] not in PAGE_SIZES or k.shape != v.shape \
@@ -126,7 +128,8 @@ class KVPlan(_Fixed):
         """Copies the three arrays to the host (which waits for the device) and raises ValueError, naming the first
         sequence, where they break a bound of the plan, of the cache or of ``total_rows`` packed rows; with
         ``for_append`` also where a sequence has more rows than tokens, or a page that is appended to is listed
-        twice."""
+        twice.  Also where a page that holds tokens (with ``for_append``: tokens before the rows) has a scale whose
+        exponent lies outside [-48, 48], which the kernels do not look for (a NaN scale is a value like others)."""
         self._fits(cache)
         table, starts, lens = (t.cpu().contiguous() for t in (self.page_table, self.row_start, self.kv_len))
         host = _lib.KVBatchParams(page_table=table.data_ptr(), table_sb=self.table_pages, row_start=starts.data_ptr(),
@@ -139,6 +142,17 @@ class KVPlan(_Fixed):
             b = bad.value
             raise ValueError("KVPlan: sequence %d (rows [%d, %d), %d tokens) breaks a bound"
                              % (b, starts[b], starts[b + 1], lens[b]) if b >= 0 else _lib.strerror(rc))
+        held = lens - starts.diff() if for_append else lens
+        listed = torch.arange(self.table_pages) * cache.page_size < held[:, None]
+        ids = torch.where(listed, table, 0).to(cache.device).long()
+        for scale in (cache.k_scale, cache.v_scale):
+            at = scale.view(torch.uint8)[ids]
+            out = ((at < 127 + EXPONENTS[0]) | (at > 127 + EXPONENTS[1])) & (at != 255)
+            out = out.any(-1).cpu() & listed
+            if out.any():
+                b, t = out.nonzero()[0].tolist()
+                raise ValueError("KVPlan: sequence %d (page %d) sees a scale outside 2^%d .. 2^%d"
+                                 % (b, table[b, t], *EXPONENTS))
 
     def _fits(self, cache: KVCache):
         if cache._index != self._index:

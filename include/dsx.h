@@ -381,7 +381,8 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
  *
  * Codes: e4m3, element (page, head, token, d) of k at k + page*k_sp + head*k_sh + token*128 + d (v likewise).
  * Scales: e8m0 (a byte x stands for 2^(x-127)), one per (page, head), at k_scale + page*ks_sp + head; the value that a
- * code stands for is code * scale.  Exponents are in [-48, 48]; byte 255 makes every row that sees the block NaN.
+ * code stands for is code * scale.  Exponents are in [-48, 48] (the kernels do not look; others give inexact results); byte
+ * 255 makes every row that sees the block NaN.
  *
  * A batch is packed row-wise: rows [row_start[b], row_start[b+1]) of q, k, v and the outputs belong to sequence b, whose
  * cache holds kv_len[b] tokens, these rows (the newest) included; token t of it lives in page

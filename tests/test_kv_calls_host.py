@@ -147,3 +147,35 @@ def test_the_workspace_is_sized_by_the_tensors_device(calls):
     calls.calls.clear()
     ops.kv_attention(torch.zeros(6, 2, 128, dtype=BF), cache, plan, split_keys=False)
     assert calls.calls == [("dsx_kv_attn", 1)]
+
+
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+def test_plan_check_looks_at_the_scales_of_pages_that_hold_tokens(name):
+    from diffsynth_engine_amd.kv_cache import KVCache, KVPlan
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    cache = KVCache.empty(6, 3, 16, "cpu")
+    # sequence 0: 20 tokens, 3 of them rows, on pages 4 and 1; sequence 1: 17 tokens, all rows, on 2 and 0
+    plan = KVPlan(i32([[4, 1, -7], [2, 0, 99]]), i32([0, 3, 20]), i32([20, 17]), max_rows=17, max_kv_len=48)
+    raw = getattr(cache, name).view(torch.uint8)
+    for page, append, attend in ((4, 0, 0), (1, 0, 0), (2, None, 1), (0, None, 1), (3, None, None), (5, None, None)):
+        for value, fits in ((78, False), (79, True), (175, True), (176, False), (254, False), (0, False), (255, True)):
+            raw[page, 2] = value
+            for for_append, bad in ((True, append), (False, attend)):
+                if fits or bad is None:
+                    plan.check(cache, 20, for_append=for_append)
+                else:
+                    with pytest.raises(ValueError, match=r"sequence %d \(page %d\)" % (bad, page)):
+                        plan.check(cache, 20, for_append=for_append)
+        raw[page, 2] = 127
+    plan.kv_len.copy_(i32([3, 17]))  # no tokens before the rows: nothing to look at
+    raw.fill_(0)
+    plan.check(cache, 20)
+    # strided scales
+    wide = torch.full((6, 2, 3), 127, dtype=torch.uint8)
+    wide[:, 1] = 0
+    args = dict(k_scale=cache.k_scale, v_scale=cache.v_scale)
+    for t in args.values():
+        t.view(torch.uint8).fill_(127)
+    args[name] = wide[:, 0].view(torch.float8_e8m0fnu)
+    plan.check(KVCache(cache.k, cache.v, **args), 20, for_append=False)
