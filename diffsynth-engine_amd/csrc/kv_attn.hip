@@ -13,9 +13,14 @@
 // O^T += V^T P^T on v_mfma_f32_16x16x32_f16: V's codes are exact in fp16, and the weights get fp16's eleven bits
 // instead of bf16's eight.  fp16's range is kept safe by the weight's unit: with e_v the exponent of the block's scale,
 //   w = exp2(s c + e_v + 14 - m),  m = running maximum of s c + e_v   (c = softmax_scale log2 e),
-// lies in (0, 2^14], multiplies the raw codes, and the row sum adds 2^-e_v w.  |e_v| <= 48 bounds what two blocks can be
-// apart to 2^96: a weight, or the factor that joins two partial sums, leaves fp32's normal range (2^-126) only for
-// tokens whose share of the softmax is below 2^-30.
+// lies in (0, 2^14] and multiplies the raw codes; the row sum adds 2^-e_v w, before w is rounded.  |e_v| <= 48 bounds what
+// two blocks can be apart to 2^96: in fp32 (row sums, factors that join partial sums) a weight leaves the normal range
+// (2^-126) only for tokens whose share of the softmax is below 2^-30.  The fp16 weight is within 2^-11 of itself or 2^-25,
+// half its smallest step: beside 2^-11 sum_j p_j |v_j| an output is off by at most
+//   2^-39 max_j(p_j 2^e_j) sum_j |code_j|   over the tokens j that the row sees (tile form: 2^-33, 2^-32 with pages of 16, 32).
+// So precision is relative to the largest p_j 2^e_j, and not to a token's share alone: beside a token of the same score in a
+// block whose scale is 2^28 (2^22) as large a weight loses bits, at 2^40 (2^34) all of them.  Weights relative to the share
+// would lose the reverse, tokens of a small share in blocks of a large scale, and those dominate the output.
 // Lane (n = lane % 16, g = lane / 16) of S^T holds query n, keys 4g .. 4g + 3 of a 16-key half: packed to fp16, the two
 // halves of a tile are the B operand of the second product as they stand.
 // A masked tile may hold NaN codes of tokens that some rows do not see: 0 * NaN must not reach those rows, so such a

@@ -318,6 +318,8 @@ __global__ __launch_bounds__(512, 2) void kv_tile_kernel(AttnArgs a, int64_t uni
       return __builtin_amdgcn_ballot_w64(mx[0] - m_ref[0] > kMoveAt || mx[1] - m_ref[1] > kMoveAt) != 0;
     };
     // New references for the wave's rows; O, the row sums and the weights `pw` that are still to be multiplied follow.
+    // (Weights that were rounded to fp16 are rounded again, 2^-10 in all: making them anew would take their scores' registers,
+    // which hold the next tile's by then.  Once at most, a tile's weights being used up in the same interval.)
     auto move = [&](const float (&mx)[2], uint32_t (&pw)[2][2][4], bool with_pw) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
