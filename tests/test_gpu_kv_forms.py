@@ -2,13 +2,14 @@
 
 A form is told from outside by the workspace that a call asks for: 520 bytes a row of a partial result, in 16- or 32-row
 columns for the streaming form, 256 rows for the tile form, two for every compute unit where all tiles are shared evenly."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 from oracle import kv_cache as okv
-from test_gpu_kv_cache import Case, ManyRows
+from test_gpu_kv_cache import PAGES, Case, ManyRows, Pool
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,97 @@ def test_weights_far_below_the_largest(dev, kind, half, page, apart):
             if apart > 12:
                 most += half * top * codes
             assert ((got[row, h] - want[row, h]).abs() <= most).all(), (row, h)
+
+
+# ------------------------------------------------------------------------------------------------ forms
+
+def workspace(cache, plan, q, window=0):
+    from diffsynth_engine_amd import _lib
+
+    P = _lib.KVAttnParams(total_rows=q.shape[0], softmax_scale=0.1, heads_q=q.shape[1], window=window)
+    return _lib.load().dsx_kv_attn_workspace_bytes(cache._ref, plan._ref, ctypes.byref(P))
+
+
+def agree(a, b, pool, plan, q, **kw):
+    """Two results of the same call, each within 2^-8 |o| + 2^-9 A of the exact one (the bound of the other tests), where
+    A = sum_j p_j |v_j| is the same attention over the codes' magnitudes."""
+    from diffsynth_engine_amd import kv_cache, ops
+
+    sizes = pool.codes[1].view(torch.uint8).bitwise_and(0x7f).view(F8)
+    cache = kv_cache.KVCache(pool.cache.k, sizes, pool.cache.k_scale, pool.cache.v_scale)
+    size = ops.kv_attention(q, cache, plan, split_keys=False, **kw).double()
+    off = (a.double() - b.double()).abs() - 2.0 ** -7 * (1 + 2.0 ** -6) * b.double().abs() - 2.0 ** -8 * (1 + 2.0 ** -6) * size
+    assert off.max().item() <= 0, off.max().item()
+
+
+def compute_units(dev):
+    return torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("batch,heads,group,rows", [
+    (66, 8, 4, 1),     # one column of 16 rows
+    (66, 8, 4, 5),     # two: 20 of 32
+    (50, 8, 1, 32),    # all 32, and sequences of 16 and fewer among them
+    (700, 8, 17, 1),   # one row in the second column; more sequences than lanes; several units a share
+    (1, 40, 7, 4),     # a share is a piece of one unit
+])
+def test_even_shares(dev, page, batch, heads, group, rows):
+    from diffsynth_engine_amd import ops
+
+    g = torch.Generator().manual_seed(batch + rows)
+    top = {1: 150000, 700: 1024}.get(batch, 16384)
+    pool = Pool(dev, heads, 64, page, seed=batch + page)
+    lens = torch.randint(0, top + 1, (batch,), generator=g).tolist()
+    lens[-1], lens[batch // 2] = top, top - 17
+    count = [min(int(r), n) for r, n in zip(torch.randint(0, rows + 1, (batch,), generator=g), lens)]
+    count[-1] = count[batch // 2] = rows
+    plan, starts, table, q = pool.batch(count, lens, group)
+    cus = compute_units(dev)
+    columns = 1 if rows * group <= 16 else 2
+    some = sorted({0, batch // 2, batch - 1} | set(range(3, batch, max(batch // 5, 1))))
+    for kw in (dict(), dict(window=top - top // 5), dict(causal=False)):
+        assert batch * heads * ((top - top // 5 if "window" in kw else top) // 32) >= 512 * cus
+        assert workspace(pool.cache, plan, q, kw.get("window", 0)) == 2 * cus * 16 * columns * 520
+        out = torch.full_like(q, 7.0)
+        ops.kv_attention(q, pool.cache, plan, out=out, **kw)
+        pool.check(out, q, starts, table, lens, only=some, **kw)
+        assert not out.isnan().any() and torch.equal(out, ops.kv_attention(q, pool.cache, plan, **kw))
+        whole = ops.kv_attention(q, pool.cache, plan, split_keys=False, **kw)  # every sequence, against the other form
+        agree(out, whole, pool, plan, q, **kw)
+
+
+@pytest.mark.parametrize("page", (16, 64))
+def test_even_shares_of_what_breaks_a_bound(dev, page):
+    from diffsynth_engine_amd import ops
+
+    pool = Pool(dev, 8, 64, page, seed=3)
+    lens = [16384, 9000, 0, 16000] * 17
+    plan, starts, table, q = pool.batch([5, 3, 2, 4] * 17, lens, 4)
+    assert workspace(pool.cache, plan, q) == 2 * compute_units(dev) * 32 * 520
+    clean = ops.kv_attention(q, pool.cache, plan)
+    assert (clean[starts[2]:starts[3]] == 0).all()
+    for which, change, back in ((1, lambda: plan.kv_len[1:2].fill_(16385), lambda: plan.kv_len[1:2].fill_(9000)),
+                                (64, lambda: plan.kv_len[64:65].fill_(-1), lambda: plan.kv_len[64:65].fill_(16384)),
+                                (3, lambda: plan.page_table[3, 7:8].fill_(-9),
+                                 lambda: plan.page_table[3, 7:8].copy_(table[3, 7:8]))):
+        keep = plan.page_table.clone()
+        change()
+        got = ops.kv_attention(q, pool.cache, plan)
+        mine = slice(starts[which], starts[which + 1])
+        assert got[mine].isnan().all()
+        got[mine] = clean[mine]
+        plan.page_table.copy_(keep)
+        back()
+        agree(got, clean, pool, plan, q)  # (lengths move the shares' ends, and with them the order of sums)
+    assert torch.equal(ops.kv_attention(q, pool.cache, plan), clean)
+
+
+def test_the_bound_of_the_many_rows_tests_means_the_tile_form(dev):
+    cus = compute_units(dev)
+    for rows, heads, group in (([1], 2, 1), ([150, 3], 2, 1), ([4, 1, 1, 4], 2, 7)):
+        c = ManyRows(dev, rows, [5000] * len(rows), heads=heads, group=group, seed=1)
+        units = len(rows) * heads * -(-c.plan.max_rows * group // 256)
+        assert units % cus and cus // (units % cus) >= 2  # some are cut, into as many pieces as fit or 79 // 8
+        pieces = min(cus // (units % cus), 79 // 8)
+        assert workspace(c.cache, c.plan, c.longer(c.q)) == units % cus * pieces * 256 * 520

@@ -179,3 +179,38 @@ def test_plan_check_looks_at_the_scales_of_pages_that_hold_tokens(name):
         t.view(torch.uint8).fill_(127)
     args[name] = wide[:, 0].view(torch.float8_e8m0fnu)
     plan.check(KVCache(cache.k, cache.v, **args), 20, for_append=False)
+
+
+@pytest.mark.parametrize("seqs,rows,heads,group,tokens,window,form", [
+    (1, 1, 12, 1, 1561, 0, (1, 12 * 6)),            # few units: equal pieces, as many as there are compute units and tiles
+    (32, 1, 8, 4, 4097, 0, None),                   # a unit for every compute unit: uncut
+    (64, 1, 8, 4, 16384, 0, (1, 512)),              # long: two partial results for every compute unit
+    (64, 1, 8, 4, 4064, 0, None), (64, 1, 8, 4, 8160, 0, (1, 512)),
+    (64, 5, 8, 4, 16384, 0, (2, 512)), (64, 5, 8, 4, 16384, 4000, None), (64, 5, 8, 4, 16384, 12000, (2, 512)),
+    (1, 1, 40, 1, 131071, 0, (1, 512)), (1, 4, 40, 7, 131072, 0, (2, 512)), (40, 32, 8, 1, 16384, 0, (2, 512)),
+    (700, 1, 8, 17, 1024, 0, (2, 512)),
+    (8, 5, 4, 7, 20000, 4096, (2, 64 * 4)),         # two blocks of two columns
+    (1, 600, 12, 1, 2048, 0, None),                 # many blocks, a short cache
+    (2, 300, 1, 1, 9001, 0, (2, 20 * 12)), (1, 300, 1, 1, 9001, 0, (2, 10 * 25)),  # many rows and still the streaming form
+    (2, 300, 7, 1, 9001, 0, (16, 28 * 9)),          # the tile form, all of its units cut
+    (1, 1560, 40, 1, 10920, 0, (16, 24 * 10)),      # and those behind a whole round
+    (1, 4680, 40, 1, 32760, 0, None),               # 760 units on 256: 248 behind two rounds, too many to cut
+    (3, 4096, 8, 4, 5001, 0, None),
+])
+def test_which_form_a_call_takes(seqs, rows, heads, group, tokens, window, form):
+    """(16-row columns of a partial result, their number) by the workspace that the call asks for; None: nothing is cut.  The
+    host's answer where no device can be asked is that of 256 compute units."""
+    import ctypes
+
+    from diffsynth_engine_amd import _lib
+
+    if torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("another number of compute units")
+    at = 1 << 20  # nothing is launched, and no pointer followed
+    C = _lib.KVCacheParams(k=at, v=at, k_scale=at, v_scale=at, k_sp=heads * 8192, k_sh=8192, v_sp=heads * 8192, v_sh=8192,
+                           ks_sp=heads, vs_sp=heads, pages=100, heads=heads, page_size=64)
+    N = _lib.KVBatchParams(page_table=at, table_sb=4096, row_start=at, kv_len=at, batch=seqs, table_pages=4096,
+                           max_rows=rows, max_kv_len=tokens)
+    P = _lib.KVAttnParams(total_rows=seqs * rows, softmax_scale=0.1, heads_q=heads * group, window=window)
+    got = _lib.load().dsx_kv_attn_workspace_bytes(ctypes.byref(C), ctypes.byref(N), ctypes.byref(P))
+    assert got == (0 if form is None else form[0] * 16 * form[1] * 520)
