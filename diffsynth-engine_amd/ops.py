@@ -805,9 +805,10 @@ def kv_attention(q: torch.Tensor, cache: KVCache, plan: KVPlan, *, causal: bool 
     2.3e38 (the kernels work with scale * log2 e).
 
     Rows of a sequence that breaks a bound of the plan become NaN (the first plan.max_rows of them if there are more), and
-    so do rows that see a token whose page number is out of range.  Rows of ``out`` behind the last sequence are left as
-    they are (and hold nothing meaningful in an ``out`` made here).  Where units of work are few, their key ranges are split over the chip through a workspace
-    allocated here (split_keys=False: never)."""
+    so do rows that see a token whose page number is out of range.  Rows that ``row_start`` does not name are left as they
+    are: those behind the last sequence, and those of a sequence whose entries are out of order or beyond the rows (they
+    hold nothing meaningful in an ``out`` made here).  Where units of work are few, their key ranges are split over the
+    chip through a workspace allocated here (split_keys=False: never)."""
     index = _kv_device("kv_attention", cache, plan, q, out)
     if q.dim() != 3:
         raise ValueError("kv_attention: q must be (rows, heads, 128)")

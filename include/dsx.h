@@ -389,8 +389,9 @@ int dsx_flow_match_euler_step(const void* latents, const void* v, float dt, void
  * page_table[b*table_sb + t / page_size].  row_start (batch+1), kv_len (batch) and page_table are int32 on the DEVICE and
  * may change between calls, replays of a captured call included; max_rows, max_kv_len, the calls' total_rows and
  * table_pages bound them and are what buffers and launches are sized by.  The kernels hold every value against its bound: a
- * sequence whose lengths break one is not appended and its rows (the first max_rows that lie in the output) leave attention
- * as NaN; a page number outside [0, pages) is not written, and rows that see a token of it become NaN.  dsx_kv_plan_check
+ * sequence whose lengths break one is not appended and its rows (the first max_rows of them) leave attention as NaN; where
+ * row_start itself is out of order or out of [0, total_rows], the sequence's rows cannot be named and are left as they are; a
+ * page number outside [0, pages) is not written, and rows that see a token of it become NaN.  dsx_kv_plan_check
  * does the same checks on the host.
  * Row and head strides of q, k, v and the outputs lie in [0, 2^31) elements.
  * Rows from row_start[batch] on belong to nobody and are left as they are.

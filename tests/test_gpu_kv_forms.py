@@ -147,3 +147,26 @@ def test_the_bound_of_the_many_rows_tests_means_the_tile_form(dev):
         assert units % cus and cus // (units % cus) >= 2  # some are cut, into as many pieces as fit or 79 // 8
         pieces = min(cus // (units % cus), 79 // 8)
         assert workspace(c.cache, c.plan, c.longer(c.q)) == units % cus * pieces * 256 * 520
+
+
+@pytest.mark.parametrize("kind,rows", [(Case, [2, 3, 1]), (Case, [20, 5, 4]), (ManyRows, [40, 30, 20])])
+def test_rows_that_cannot_be_named_and_rows_beyond_the_bound(dev, kind, rows):
+    """More rows than the plan's bound: that many become NaN.  Entries out of order or out of range: left as they are."""
+    from diffsynth_engine_amd import kv_cache, ops
+
+    c = kind(dev, rows, [200, 190, 180], page=32, seed=41)
+    q = c.longer(c.q) if kind is ManyRows else c.q.to(dev)
+    clean = ops.kv_attention(q, c.cache, c.plan)
+    s, bound, total = c.starts, c.plan.max_rows, q.shape[0]
+
+    def run(starts):
+        plan = kv_cache.KVPlan(c.plan.page_table, torch.tensor(starts, dtype=torch.int32, device=dev), c.plan.kv_len,
+                               max_rows=bound, max_kv_len=200)
+        out = torch.full_like(q, 7.0)
+        return ops.kv_attention(q, c.cache, plan, out=out)
+
+    for starts in ([s[0], s[1], total + 1, s[3]], [s[0], s[1], -2, s[3]], [s[0], s[1], s[1] - 1, s[1] - 1]):
+        got = run(starts)
+        assert torch.equal(got[:s[1] - 1], clean[:s[1] - 1]) and (got[s[1]:] == 7).all()
+    got = run([0, 0, bound + 1, bound + 1])
+    assert got[:bound].isnan().all() and (got[bound:] == 7).all()
