@@ -722,6 +722,7 @@ def _kv_call(fn, what: str, index: int, *args):
 
 
 def _kv_norm_weight(w: torch.Tensor) -> torch.Tensor:
+    """RMSNorm weights as the kernels take them: bf16 (rounded to it as in rmsnorm_rope), aligned."""
     if w.numel() != HEAD_DIM:
         raise ValueError("kv_append: RMSNorm weights have 128 entries")
     if w.dtype != _BF16 or not w.is_contiguous():
@@ -738,8 +739,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
     k, v: (rows, cache.heads, 128) bf16, q: (rows, heads, 128) bf16; unit stride in the last dim, other strides in
     multiples of 8 (slices of one packed projection are fine).  k gets RMSNorm per head (k_norm_w (128,), optional) and
     the rotation of its position's row of ``rope`` (fp32 (B|1, >= plan.max_kv_len, 64, 2) (cos, sin), optional), q the
-    same with q_norm_w; a row's position is its token number in its sequence.  fp32 throughout, rounded once: k and v
-    to e4m3 with one power-of-two scale per (page, head) block, q to bf16.
+    same with q_norm_w; a row's position is its token number in its sequence.  The weights are bf16, as everywhere in this
+    module (others are rounded to it first: to within 2^-8 of itself); from there on fp32 throughout, rounded
+    once: k and v to e4m3 with one power-of-two scale per (page, head) block, q to bf16.
 
     A block that keeps earlier tokens never lowers its scale; when it has to grow, the kept codes are rounded to the new
     one.  Infinities saturate, NaN stays NaN.  Appending the same rows at the same positions again changes nothing.

@@ -170,3 +170,17 @@ def test_rows_that_cannot_be_named_and_rows_beyond_the_bound(dev, kind, rows):
         assert torch.equal(got[:s[1] - 1], clean[:s[1] - 1]) and (got[s[1]:] == 7).all()
     got = run([0, 0, bound + 1, bound + 1])
     assert got[:bound].isnan().all() and (got[bound:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64])
+def test_norm_weights_of_other_types_are_rounded_to_bf16_first(dev, dtype):
+    from diffsynth_engine_amd import ops
+
+    w = (1 + 0.2 * torch.randn(128, generator=torch.Generator().manual_seed(2))).to(dtype).to(dev)
+    got = []
+    for weight in (w, w.bfloat16(), torch.cat((w[:1], w)).bfloat16()[1:]):  # the last: aligned to an element only
+        c = Case(dev, [3, 20], [40, 50], group=2, page=16, seed=5)
+        out = ops.kv_append(c.k.to(dev), c.v.to(dev), c.cache, c.plan, k_norm_w=weight, q=c.q.to(dev),
+                            q_norm_w=weight)
+        got.append([out] + [t.view(torch.uint8) for t in (c.cache.k, c.cache.k_scale)])
+    assert all(torch.equal(a, b) for x in got[1:] for a, b in zip(got[0], x))
