@@ -657,6 +657,9 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   //    512: 14 against 25; 4 x 40, group 7, 3900: 36 against 43; but 1 x 100, 40 heads, 16384: 114 against 80).
   // The rest is the tile form's, which loads a key once for 256 rows: at two blocks a compute unit it wins or draws (1 x
   // 390, 30 heads, 2048 tokens: 42 against 43; 3900: 54 against 66).
+  // All of this was measured on batches whose sequences have about as many rows each: the rule knows only the most.  4096
+  // rows over 4096 tokens and 63 x 1 over 16384, 32 / 8 heads: 2250 us in one call, all of it in the tile form, 146 and 296
+  // in two; 64 over 16384 and 63 x 1: 626 against 42 + 297.
   const int64_t blocks = (packed + 31) / 32, wgs = blocks * n.batch * c.heads;
   const bool stream = blocks <= 1 || (blocks <= 2 && (wgs <= cus || span >= 4096)) ||
                       (wgs <= cus && (2 * wgs <= cus || span < 4096));

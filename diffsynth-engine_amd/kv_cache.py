@@ -42,7 +42,8 @@ class KVCache(_Fixed):
     """Codes ``k``, ``v``: (pages, heads, page_size, 128) e4m3, any page and head strides that are multiples of 16, each
     (page, head) block contiguous.  Scales ``k_scale``, ``v_scale``: (pages, heads) e8m0, heads contiguous, from 2^-48 to
     2^48 (or NaN) wherever a token lies: others give inexact results, and nothing but ``KVPlan.check`` looks for them.  A
-    value is code * scale.  The tensors stay the caller's and are used in place; which they are is fixed when the cache is made."""
+    value is code * scale.  The tensors stay the caller's and are used in place; which they are is fixed when the cache is
+    made."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] not in PAGE_SIZES or k.shape != v.shape \
@@ -93,7 +94,9 @@ class KVPlan(_Fixed):
 
     page_table (B, P), row_start (B + 1), kv_len (B): int32 on one device.  Table entries that no token needs may hold
     anything.  max_rows, max_kv_len: no sequence will have more rows in a call, or more tokens.  They size launches
-    (and, with kv_len, how attention splits its work), so they should be near what is used.
+    (and, with kv_len, how attention splits its work), so they should be near what is used.  Nothing else about the rows is
+    known to the host: every sequence is worked on as if it had max_rows of them.  Prompts and sequences with a token or a
+    few belong in plans and calls of their own (``ops.kv_attention`` has the figures).
 
     The arrays are not read on the host.  What breaks a bound on the device is left out there: see ``check`` and the
     notes of ``ops.kv_append`` and ``ops.kv_attention``."""

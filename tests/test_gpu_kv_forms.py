@@ -184,3 +184,21 @@ def test_norm_weights_of_other_types_are_rounded_to_bf16_first(dev, dtype):
                             q_norm_w=weight)
         got.append([out] + [t.view(torch.uint8) for t in (c.cache.k, c.cache.k_scale)])
     assert all(torch.equal(a, b) for x in got[1:] for a, b in zip(got[0], x))
+
+
+def test_a_prompt_beside_single_rows_is_right_together_and_apart(dev):
+    """Slices of one plan's arrays make the plans of two calls."""
+    from diffsynth_engine_amd import kv_cache, ops
+
+    pool = Pool(dev, 8, 64, 64, seed=11)
+    rows, lens = [700] + [1] * 20, [900] + [3000 - 100 * i for i in range(20)]
+    plan, starts, table, q = pool.batch(rows, lens, 4)
+    whole = ops.kv_attention(q, pool.cache, plan)
+    pool.check(whole, q, starts, table, lens, only=(0, 1, 7, 20))
+    for a, b in ((0, 1), (1, 21)):
+        first = starts[a]
+        part = kv_cache.KVPlan(plan.page_table[a:b], plan.row_start[a:b + 1] - first, plan.kv_len[a:b],
+                               max_rows=max(rows[a:b]), max_kv_len=max(lens[a:b]))
+        own = slice(first, starts[b])
+        got = ops.kv_attention(q[own], pool.cache, part)
+        agree(got, whole[own], pool, part, q[own])
