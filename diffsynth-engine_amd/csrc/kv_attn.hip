@@ -28,7 +28,7 @@
 //
 // Bound: HBM, 256 bytes a token and cache head for a handful of flops each; codes go from memory to registers in whole
 // 128-byte lines and nothing is staged.  A read of the same pages without any arithmetic reaches 6.0 TB/s; 1 x 131071
-// tokens, 40 heads: 225 us and 5 for the join (5.8 TB/s); 64 sequences to 16384 tokens, 8 heads: 276 + 5 us (5.8 TB/s).
+// tokens, 40 heads: 228 us and 5 for the join (5.8 TB/s); 64 sequences to 16384 tokens, 8 heads: 276 + 5 us (5.8 TB/s).
 // Eight waves of 228 to 256 registers fill a compute unit (with four of them the 131071 tokens took 282 us instead of 258).
 // Short caches are bound by the chain launch -> lengths -> page numbers -> scales and codes -> products -> join of the
 // waves: 1 x 1561 tokens, 12 heads: 7.1 us and 3.5 for the join of the pieces.  Hence first pages beside the lengths, codes
@@ -677,9 +677,10 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
     // workgroup per unit and its uneven end: 64 x 16384 tokens, 8 heads (1024 tiles): 280 against 305 us; 32 x 16384 (512):
     // 168 against 178; 32 x 8192 (256): 93 against 86; 32 x 4097 (129): 58 against 44.
     // Fewer units than compute units are cut into equal pieces, as many as there are compute units and tiles for the waves,
-    // from four tiles a wave on: 1 x 1561 tokens, 12 heads (six pieces): 11.6 against 14.5 us, 1000 tokens: 10.6 against
-    // 12.1; below that the join costs more than it saves: 4 x 5 rows, 4 heads, 800 tokens: 15.4 against 14.9, 500: 14.0
-    // against 12.6.  Fewer, longer pieces bring nothing (1561 tokens in three: 12.7).
+    // from four tiles a wave on: replayed from a graph, 1 x 1561 tokens, 12 heads (six pieces): 10.1 against 13.1 us, 1000
+    // tokens: 9.2 against 10.7, 4 x 5 rows, 4 heads, 1000 tokens: 13.5 against 14.7; below that the join costs more than it
+    // saves (cut at 800 tokens: 15.4 against 14.9, at 500: 14.0 against 12.6, before later steps).  Fewer, longer pieces
+    // bring nothing (1561 tokens in three: 12.7 against 11.6, at the same time).
     const int64_t load = r.units * tiles / cus;
     if (load >= 512 && r.nqb == 1 && r.units * tiles < (1ll << 30)) {
       r.share = cus;

@@ -15,10 +15,13 @@
 //    some of them would leave fp16 (2^15) does m become the maximum so far.  A tile that does not move it costs no
 //    rescaling of O, and where a tile has one scale (pages of 64 and more) no look at its scores' maximum either: the row
 //    sums, which are needed anyway, tell.
-// Bound: the matrix pipe with the vector work and LDS beside it: 2048 cycles of matrix instructions a tile and SIMD, some 2100
-// of vector instructions, some 2100 of LDS, 3600 measured.  4680 rows over 32760 tokens, 40 heads: 2.40 ms, 1310 TFLOP/s of
-// the two products (a large bf16 matrix product: 1525; the framework's attention over bf16 keys of the same size: 1125).  On
-// that case (2.65 ms then), in copies with work left out: without q's low term 8 % less, without exponentials 4 %, without
+// Bound: the matrix pipe with the vector work and LDS beside it: 2050 cycles of matrix instructions a tile and SIMD, 1960 of
+// vector issue, 1170 of LDS reads and writes, by counters; 3380 measured over 512 tiles (at 1.85 of 2.4 GHz in that run).
+// 4680 rows over 32760 tokens, 40 heads: 2.41 to 2.57 ms by machine, 1222 to 1303 TFLOP/s of the two products (a large bf16
+// matrix product: 1525; the framework's attention over bf16 keys of the same size: 1125 to 1250); pages of 16: 2.67 ms
+// (236 vector instructions a wave and tile instead of 194).  3 prompts of 4096 rows, 37 tiles a unit: 0.325 ms and 3980 cycles
+// a tile, with its share of the units' beginnings and ends.  On the
+// first case (2.65 ms then), in copies with work left out: without q's low term 8 % less, without exponentials 4 %, without
 // V's conversion 5 %, without the scores' maximum 7 % (of which looking at the row sums instead got 5).  Exponentials in
 // other places (two to six in front of the first product, 8 to 20 in the second stage), three or four fragments of V ahead:
 // no change beyond noise.
