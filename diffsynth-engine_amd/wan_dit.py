@@ -86,11 +86,15 @@ class WanFrameCache:
     def bytes(self) -> int:
         return sum(t.numel() for c in self.layers for t in (c.k, c.v, c.k_scale, c.v_scale))
 
-    def plan(self, first: int, frames: int) -> KVPlan:
-        """The batch of a call that computes frames [first, first + frames)."""
+    def check(self, first: int, frames: int) -> None:
+        """ValueError unless frames [first, first + frames) continue what is held, or replace a part of it, and fit."""
         if not 0 <= first <= self.frames or frames < 1 or first + frames > self.max_frames:
             raise ValueError("WanFrameCache: frames [%d, %d) do not continue the %d that are held (of %d at most)"
                              % (first, first + frames, self.frames, self.max_frames))
+
+    def plan(self, first: int, frames: int) -> KVPlan:
+        """The batch of a call that computes frames [first, first + frames)."""
+        self.check(first, frames)
         rows, tokens = frames * self.h * self.w, (first + frames) * self.h * self.w
         starts = torch.arange(0, (self.batch + 1) * rows, rows, dtype=torch.int32, device=self.table.device)
         lens = torch.full((self.batch,), tokens, dtype=torch.int32, device=self.table.device)
@@ -311,12 +315,13 @@ class WanDiTRunner:
                 raise ValueError("the cache was made for a batch of %d, %d x %d tokens a frame and %d blocks"
                                  % (cache.batch, cache.h, cache.w, len(cache.layers)))
             first = first_frame // pf
-            plan = cache.step(first, f)
+            cache.check(first, f)
         patches = x.to(bf).view(B, C, f, pf, h, ph, w, pw).permute(0, 2, 4, 6, 1, 3, 5, 7)
         hs = self._linear_bf16(patches.reshape(B, f * h * w, C * pf * ph * pw), "patch_embedding")
         rope = self.rope_table(f, h, w, first=first)
         ctx_q = self.quantise_context(ctx)
-        if cache is not None:
+        if cache is not None:  # (a call that fails in front of the blocks leaves it as it was)
+            plan = cache.step(first, f)
             cache.frames = first  # (should a block raise: what was there from here on is overwritten in part)
         for i in range(cfg["num_layers"]):
             hs = self.block(i, hs, ctx, t_mod, rope, ctx_q, None if cache is None else (cache.layers[i], plan))

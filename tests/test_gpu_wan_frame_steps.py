@@ -98,3 +98,25 @@ def test_a_step_that_raises_leaves_no_frames_that_it_overwrote(dev, monkeypatch)
     with pytest.raises(ValueError):  # frame 1 is not there any more
         R(x[:, :, 2:].contiguous(), ctx, t, cache=cache, first_frame=2)
     assert torch.equal(R(part, ctx, t, cache=cache, first_frame=1), R(part, ctx, t, cache=twin, first_frame=1))
+
+
+def test_a_refused_call_leaves_the_run_in_progress_as_it_was(dev):
+    R = _runner(dev)
+    x, ctx, t = _inputs(dev, 3)
+    once, often = (R.frame_cache(3, 12, 14) for _ in range(2))
+    weights = [R.vec["blocks.%d.self_attn.norm_k.weight" % i] for i in range(2)]
+    for c in (once, often):
+        R(x[:, :, :1].contiguous(), ctx, t, cache=c)
+        R(x[:, :, 1:2].contiguous(), ctx, t, cache=c, first_frame=1)
+    part = x[:, :, 2:].contiguous()
+    for w in weights:
+        w.mul_(2.0 ** 14)
+    R(part, ctx, t, cache=often, first_frame=2)  # a step that is thrown away
+    for w in weights:
+        w.div_(2.0 ** 14)
+    state = _state(often)
+    for bad in (dict(context=ctx[..., :100]), dict(x=part[:, :8])):  # a text width and a channel number that do not fit
+        with pytest.raises(Exception):
+            R(**{**dict(x=part, context=ctx, timestep=t, cache=often, first_frame=1), **bad})
+    assert often.frames == 3 and all(torch.equal(a, b) for a, b in zip(state, _state(often)))
+    assert torch.equal(R(part, ctx, t, cache=once, first_frame=2), R(part, ctx, t, cache=often, first_frame=2))
