@@ -661,8 +661,10 @@ Plan make_plan(const dsx_kv_cache& c, const dsx_kv_batch& n, const dsx_kv_attn_p
   // rows over 4096 tokens and 63 x 1 over 16384, 32 / 8 heads: 2250 us in one call, all of it in the tile form, 146 and 296
   // in two; 64 over 16384 and 63 x 1: 626 against 42 + 297.
   const int64_t blocks = (packed + 31) / 32, wgs = blocks * n.batch * c.heads;
-  const bool stream = blocks <= 1 || (blocks <= 2 && (wgs <= cus || span >= 4096)) ||
-                      (wgs <= cus && (2 * wgs <= cus || span < 4096));
+  const bool one_each = wgs <= cus, long_cache = span >= 4096;
+  const bool stream = blocks <= 1   ? true
+                      : blocks == 2 ? one_each || long_cache
+                                    : one_each && (2 * wgs <= cus || !long_cache);
   r.nq = packed <= 16 ? 1 : stream ? 2 : 0;
   r.block_rows = r.nq ? 16 * r.nq : kTileRows;
   r.nqb = (int)((packed + r.block_rows - 1) / r.block_rows);
