@@ -92,8 +92,9 @@ class KVPlan(_Fixed):
     """A packed batch: rows [row_start[b], row_start[b + 1]) of q, k and v are the newest tokens of sequence b, which
     has kv_len[b] tokens with them; token t of it is in page page_table[b, t // page_size].
 
-    page_table (B, P), row_start (B + 1), kv_len (B): int32 on one device.  Table entries that no token needs may hold
-    anything.  max_rows, max_kv_len: no sequence will have more rows in a call, or more tokens.  They size launches
+    page_table (B, P), row_start (B + 1), kv_len (B): int32 on one device.  Table entries that no row sees a
+    token of may hold anything: those behind a sequence's end and, for attention with a window, pages that lie in front of
+    every row's (``check`` knows of no window and reports these).  max_rows, max_kv_len: no sequence will have more rows in a call, or more tokens.  They size launches
     (and, with kv_len, how attention splits its work), so they should be near what is used.  Nothing else about the rows is
     known to the host: every sequence is worked on as if it had max_rows of them.  Prompts and sequences with a token or a
     few belong in plans and calls of their own (``ops.kv_attention`` has the figures).

@@ -202,3 +202,33 @@ def test_a_prompt_beside_single_rows_is_right_together_and_apart(dev):
         own = slice(first, starts[b])
         got = ops.kv_attention(q[own], pool.cache, part)
         agree(got, whole[own], pool, part, q[own])
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("rows,lens,group,window", [
+    ([1], [3000], 4, 500),             # one column
+    ([5, 2], [3000, 1700], 7, 333),    # two
+    ([40, 9], [3000, 500], 1, 64),
+    ([700, 300], [2500, 2000], 20, 900),  # the tile form
+    ([1] * 66, [16384 - 7 * i for i in range(66)], 4, 13000),  # even shares
+])
+def test_pages_in_front_of_every_window_are_not_looked_at(dev, page, rows, lens, group, window):
+    """A program with a window gives such pages to others: their table entries may hold anything."""
+    from diffsynth_engine_amd import ops
+
+    pool = Pool(dev, 8, 64, page, seed=page + len(rows))
+    plan, starts, table, q = pool.batch(rows, lens, group)
+    if len(rows) == 66:
+        assert workspace(pool.cache, plan, q, window) == 2 * compute_units(dev) * 16 * 520
+    clean = ops.kv_attention(q, pool.cache, plan, window=window)
+    pool.check(clean, q, starts, table, lens, window=window, only=(0, len(rows) - 1))
+    pool.cache.k.view(torch.uint8)[0, :, :, ::5] = 0x7f  # what stands in for a page out of range: NaN here
+    pool.cache.v.view(torch.uint8)[0, :, :, ::5] = 0xff
+    table = torch.where(table == 0, 1, table)
+    plan.page_table.copy_(table)
+    clean = ops.kv_attention(q, pool.cache, plan, window=window)
+    assert not clean.isnan().any()
+    for bad in (-1, 10 ** 9, 0):
+        for b, (r, n) in enumerate(zip(rows, lens)):
+            plan.page_table[b, :max(n - r + 1 - window, 0) // page] = bad
+        assert torch.equal(ops.kv_attention(q, pool.cache, plan, window=window), clean), bad
