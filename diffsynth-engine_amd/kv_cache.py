@@ -92,12 +92,12 @@ class KVPlan(_Fixed):
     """A packed batch: rows [row_start[b], row_start[b + 1]) of q, k and v are the newest tokens of sequence b, which
     has kv_len[b] tokens with them; token t of it is in page page_table[b, t // page_size].
 
-    page_table (B, P), row_start (B + 1), kv_len (B): int32 on one device.  Table entries that no row sees a
-    token of may hold anything: those behind a sequence's end and, for attention with a window, pages that lie in front of
-    every row's (``check`` knows of no window and reports these).  max_rows, max_kv_len: no sequence will have more rows in a call, or more tokens.  They size launches
-    (and, with kv_len, how attention splits its work), so they should be near what is used.  Nothing else about the rows is
-    known to the host: every sequence is worked on as if it had max_rows of them.  Prompts and sequences with a token or a
-    few belong in plans and calls of their own (``ops.kv_attention`` has the figures).
+    page_table (B, P), row_start (B + 1), kv_len (B): int32 on one device.  Table entries that no row sees a token of may
+    hold anything: those behind a sequence's end and, for attention with a window, pages that lie in front of every row's
+    (``check`` knows of no window and reports these).  max_rows, max_kv_len: no sequence will have more rows in a call, or
+    more tokens.  They size launches (and, with kv_len, how attention splits its work), so they should be near what is used.
+    Nothing else about the rows is known to the host: every sequence is worked on as if it had max_rows of them.  Prompts
+    and sequences with a token or a few belong in plans and calls of their own (``ops.kv_attention`` has the figures).
 
     The arrays are not read on the host.  What breaks a bound on the device is left out there: see ``check`` and the
     notes of ``ops.kv_append`` and ``ops.kv_attention``."""
