@@ -17,7 +17,8 @@
 // two blocks can be apart to 2^96: in fp32 (row sums, factors that join partial sums) a weight leaves the normal range
 // (2^-126) only for tokens whose share of the softmax is below 2^-30.  The fp16 weight is within 2^-11 of itself or 2^-25,
 // half its smallest step: beside 2^-11 sum_j p_j |v_j| an output is off by at most
-//   2^-39 max_j(p_j 2^e_j) sum_j |code_j|   over the tokens j that the row sees (tile form: 2^-33, 2^-32 with pages of 16, 32).
+//   2^-39 max_j(p_j 2^e_j) sum_j |code_j|   over the tokens j that the row sees
+// (tile form: 2^-33; with pages of 16 and 32, where a weight may be rounded twice: 2^-32, beside 2^-10 sum_j p_j |v_j|).
 // So precision is relative to the largest p_j 2^e_j, and not to a token's share alone: beside a token of the same score in a
 // block whose scale is 2^28 (2^22) as large a weight loses bits, at 2^40 (2^34) all of them.  Weights relative to the share
 // would lose the reverse, tokens of a small share in blocks of a large scale, and those dominate the output.

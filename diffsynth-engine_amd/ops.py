@@ -740,8 +740,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, plan: KVPlan, *,
     multiples of 8 (slices of one packed projection are fine).  k gets RMSNorm per head (k_norm_w (128,), optional) and
     the rotation of its position's row of ``rope`` (fp32 (B|1, >= plan.max_kv_len, 64, 2) (cos, sin), optional), q the
     same with q_norm_w; a row's position is its token number in its sequence.  The weights are bf16, as everywhere in this
-    module (others are rounded to it first: to within 2^-8 of itself); from there on fp32 throughout, rounded
-    once: k and v to e4m3 with one power-of-two scale per (page, head) block, q to bf16.
+    module (others are rounded to it first, to within 2^-8 of themselves); from there on fp32 throughout, rounded once: k
+    and v to e4m3 with one power-of-two scale per (page, head) block, q to bf16.
 
     A block that keeps earlier tokens never lowers its scale; when it has to grow, the kept codes are rounded to the new
     one.  Infinities saturate, NaN stays NaN.  Appending the same rows at the same positions again changes nothing.

@@ -282,9 +282,10 @@ class WanDiTRunner:
 
         ``cache``: x holds the latent frames [first_frame, first_frame + x.shape[2]) of a longer video.  They attend to
         one another and to the frames in front of them, as the cache has them; their own keys and values replace what it
-        holds from first_frame on, as if no step before had written there.  A denoising loop calls this with the same first_frame for every step of a run of
-        frames, and goes on behind them when they are done; what stays in the cache is the last call's, so whoever wants
-        the finished frames there, and not those of the last noisy step, calls once more with them."""
+        holds from first_frame on, as if no step before had written there.  A denoising loop calls this with the same
+        first_frame for every step of a run of frames, and goes on behind them when they are done; what stays in the cache
+        is the last call's, so whoever wants the finished frames there, and not those of the last noisy step, calls once
+        more with them."""
         cfg = self.cfg
         d = cfg["dim"]
         pf, ph, pw = cfg["patch_size"]

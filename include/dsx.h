@@ -450,8 +450,9 @@ int dsx_kv_append(const dsx_kv_cache* cache, const dsx_kv_batch* batch, const ds
  * last `window` when window > 0.  A row that sees nothing gives zeros (causal rows with negative positions; kv_len 0).
  * Query head h reads cache head h / (heads_q / heads); heads_q is a multiple of heads.
  * Softmax and sums in fp32.  q is used as the exact sum of two scaled e4m3 terms (each element to 2^-22 of its row's
- * largest), the weights p_j 2^e_j (e_j: exponent of v's block) enter the second product as fp16, relative to the row's
- * largest: 2^-11 of each, and in all 2^-32 max_j(p_j 2^e_j) sum_j |code_j| at most for those that lie far below it.  A q row with a non-finite element gives NaN.
+ * largest).  The weights p_j 2^e_j (e_j: exponent of v's block) enter the second product as fp16, relative to the row's
+ * largest: each is off by 2^-10 of itself at most, and those that lie far below the largest by
+ * 2^-32 max_j(p_j 2^e_j) sum_j |code_j| in all.  A q row with a non-finite element gives NaN.
  * q, out: (total_rows, heads_q, 128) bf16 by row and head strides (multiples of 8, 16-byte aligned); out may be q
  * itself, and otherwise shares no memory with it.
  * workspace: dsx_kv_attn_workspace_bytes(...) bytes, 16-byte aligned, lets the key range be split over the compute units
